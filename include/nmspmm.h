@@ -322,6 +322,63 @@ int nmspmm_tile_wave_sets(int M, int N, int W, int kept, int Ns, int split_k);
 int nmspmm_gemm_auto(const float* A, const float* B, const int32_t* D, const int32_t* column_info,
                      float* C, int M, int N, int K, int W, float sparsity, void* stream);
 
+/* ---- operands in 4 bits ---------------------------------------------------------------------- */
+
+/* No counterpart in the reference, whose kept values are fp32.  The kept values of an N:M-compressed
+ * operand (or, with n == m, of an ordinary dense one) as whole numbers 0 .. 15, with a scale and a
+ * zero point for each group of `group` kept rows of a column:
+ *     B[r][c] = scale[r / group][c] * (code[r][c] - zero[r / group][c])
+ * for kept row r of W = K * n / m and column c of N.  Decoding reads an operand once per token, and it
+ * is what bounds it: 4 bits, and 4 bytes a group, in place of 32 bits.
+ * Patterns: n == m (dense: any K and N), or n in {1, 2, 4, 8} kept rows in every window of m = 2 n, 4 n
+ * or 8 n (K % m == 0, N % 32 == 0, one index pattern per 32 columns, as everywhere in this library);
+ * group 32, 64 or 128; K below 2^30, N up to 2^21.
+ * The buffers are made once, by nmspmm_q4_quantize_device or nmspmm_q4_pack_device, in the layout that
+ * the kernels read; they belong to the caller, who gives them the sizes that the three functions below
+ * return and 16-byte alignment.  `bias` (float[N] or NULL) is added by nmspmm_q4_linear.  The struct is
+ * read during the call only. */
+typedef struct nmspmm_q4_operand {
+    void* codes;        /* nmspmm_q4_codes_bytes */
+    void* meta;         /* nmspmm_q4_meta_bytes: scales and zero points */
+    void* row_offsets;  /* nmspmm_q4_row_offsets_bytes: which rows are kept; NULL when n == m */
+    const float* bias;
+    int K, N, n, m, group;
+} nmspmm_q4_operand;
+
+/* Bytes of the three buffers; 0 for invalid arguments (and row offsets of a dense operand). */
+size_t nmspmm_q4_codes_bytes(int K, int N, int n, int m);
+size_t nmspmm_q4_meta_bytes(int K, int N, int n, int m, int group);
+size_t nmspmm_q4_row_offsets_bytes(int K, int N, int n, int m);
+
+/* Fills the operand's buffers from fp32 values: dBT[W][N] and, when n < m, dDT[W][N/32] as
+ * nmspmm_compress_device writes them (dDT NULL otherwise).  Per group of a column:
+ *   symmetric (flags 0): zero = 8, scale the smallest number of 20 significant bits with 7 * scale >= max |b|;
+ *   NMSPMM_Q4_ASYMMETRIC: 15 * scale >= max(b, 0) - min(b, 0), zero = -min(b, 0) / scale to the nearest;
+ *   code = b / scale to the nearest whole number (ties to even, of the exact quotient) plus zero, held
+ *   in 0 .. 15.
+ * A group that holds a NaN or an infinity gets a NaN scale.  A row number outside its window makes that
+ * kept value zero; the numbers of a window are expected to be distinct.  Asynchronous on `stream`. */
+#define NMSPMM_Q4_ASYMMETRIC 1u
+int nmspmm_q4_quantize_device(const float* dBT, const int32_t* dDT, const nmspmm_q4_operand* op,
+                              unsigned flags, void* stream);
+/* The same from codes that exist already (an imported checkpoint): d_codes[W][N], one code per byte
+ * (the low four bits count), d_scales[ceil(W / group)][N] (kept to 20 significant bits: scales that
+ * were 16-bit floats are exact), d_zeros like d_scales, one 0 .. 15 per byte, or NULL for 8. */
+int nmspmm_q4_pack_device(const uint8_t* d_codes, const float* d_scales, const uint8_t* d_zeros,
+                          const int32_t* dDT, const nmspmm_q4_operand* op, void* stream);
+/* The operand as the dense fp32 matrix dB[K][N], zeros where rows were not kept (exact). */
+int nmspmm_q4_expand_device(const nmspmm_q4_operand* op, float* dB, void* stream);
+
+/* y[M][N] = x[M][K] B + bias: rows of x are ldx elements apart (ldx >= K), rows of y ldy (>= N), both of
+ * `type`; sums in fp32, one rounding at the end.  M == 0 does nothing.  fp32 activations are multiplied
+ * exactly (three bf16 pieces each), so the result is as near as an fp32 product's.  A row of x that
+ * holds an infinity or a NaN, or magnitudes beyond 2^100, gives a row of NaN.  x and y must not overlap.  Results do not
+ * depend on what runs beside the call and repeat bit for bit.  No library state: any streams and threads;
+ * may be captured into a HIP graph. */
+typedef enum nmspmm_type { NMSPMM_F32 = 0, NMSPMM_BF16 = 1, NMSPMM_F16 = 2 } nmspmm_type;
+int nmspmm_q4_linear(const nmspmm_q4_operand* op, const void* x, long long ldx, void* y,
+                     long long ldy, int M, int type, void* stream);
+
 /* Frees what the library keeps per device: the cached split-K workspaces and the staging buffer
  * of the host-pointer preprocessing forms; forgets every attached row list. */
 int nmspmm_release(void);

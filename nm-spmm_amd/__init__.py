@@ -24,6 +24,17 @@ STREAM_B = 2    # flag of spmm_ex: B is loaded with the non-temporal hint (decod
 DECODE_SPLIT = 4  # flag of spmm_ex: the decode kernel may cut reductions across workgroups (library scratch)
 
 
+Q4_ASYMMETRIC = 1  # flag of q4_quantize_device: a zero point for each group
+F32, BF16, F16 = 0, 1, 2  # nmspmm_type
+
+
+class Q4Operand(ctypes.Structure):
+    """nmspmm_q4_operand: device pointers and geometry of an operand in 4 bits."""
+    _fields_ = [("codes", ctypes.c_void_p), ("meta", ctypes.c_void_p), ("row_offsets", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("K", ctypes.c_int), ("N", ctypes.c_int), ("n", ctypes.c_int), ("m", ctypes.c_int),
+                ("group", ctypes.c_int)]
+
+
 class NmSpmmError(RuntimeError):
     def __init__(self, fn, status):
         self.status = status
@@ -83,6 +94,14 @@ def lib():
         L.nmspmm_tile_wave_sets.argtypes = [c_int] * 6
         L.nmspmm_device_figures.argtypes = [ip, ip, ctypes.POINTER(ctypes.c_double)]
         L.nmspmm_gemm_auto.argtypes = [c_void_p] * 5 + [c_int] * 4 + [c_float, c_void_p]
+        op = ctypes.POINTER(Q4Operand)
+        L.nmspmm_q4_codes_bytes.restype = L.nmspmm_q4_meta_bytes.restype = L.nmspmm_q4_row_offsets_bytes.restype = c_size_t
+        L.nmspmm_q4_codes_bytes.argtypes = L.nmspmm_q4_row_offsets_bytes.argtypes = [c_int] * 4
+        L.nmspmm_q4_meta_bytes.argtypes = [c_int] * 5
+        L.nmspmm_q4_quantize_device.argtypes = [c_void_p, c_void_p, op, ctypes.c_uint, c_void_p]
+        L.nmspmm_q4_pack_device.argtypes = [c_void_p] * 4 + [op, c_void_p]
+        L.nmspmm_q4_expand_device.argtypes = [op, c_void_p, c_void_p]
+        L.nmspmm_q4_linear.argtypes = [op, c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p]
         L.nmspmm_release.restype = c_int
         _lib = L
     return _lib
@@ -255,6 +274,62 @@ def gemm_high_sparsity(tile, A, B, D, cinfo, C, M, N, K, W, sparsity, split_k=1)
     _check("nmspmm_gemm_high_sparsity",
            lib().nmspmm_gemm_high_sparsity(tile, _ptr(A), _ptr(B), _ptr(D), _ptr(cinfo), _ptr(C), M, N, K, W,
                                            sparsity, split_k, _stream()))
+
+
+# ---- operands in 4 bits: the struct is made by q4_operand from torch tensors ---------------------------
+
+def q4_codes_bytes(K, N, n=1, m=1):
+    return lib().nmspmm_q4_codes_bytes(K, N, n, m)
+
+
+def q4_meta_bytes(K, N, n=1, m=1, group=128):
+    return lib().nmspmm_q4_meta_bytes(K, N, n, m, group)
+
+
+def q4_row_offsets_bytes(K, N, n=1, m=1):
+    return lib().nmspmm_q4_row_offsets_bytes(K, N, n, m)
+
+
+def q4_operand(codes, meta, row_offsets, K, N, n=1, m=1, group=128, bias=None):
+    """The struct the q4_* functions take; the caller keeps the tensors alive as long as it is used."""
+    for name, t, need in (("codes", codes, q4_codes_bytes(K, N, n, m)), ("meta", meta, q4_meta_bytes(K, N, n, m, group)),
+                          ("row_offsets", row_offsets, q4_row_offsets_bytes(K, N, n, m)), ("bias", bias, 4 * N)):
+        if t is not None and t.numel() * t.element_size() < need:
+            raise ValueError("q4_operand: %s holds %d bytes, the shape arguments need %d"
+                             % (name, t.numel() * t.element_size(), need))
+    at = [None if t is None else t.data_ptr() for t in (codes, meta, row_offsets, bias)]
+    return Q4Operand(*at, K, N, n, m, group)
+
+
+def q4_quantize_device(dBT, dDT, op, flags=0):
+    """float32[W][N] (and int32[W][N/32] when n < m) -> the operand's buffers."""
+    W = op.K // max(op.m, 1) * op.n
+    _need("q4_quantize_device", dBT=(dBT, W * op.N), dDT=(dDT, W * (op.N // 32)))
+    _check("nmspmm_q4_quantize_device",
+           lib().nmspmm_q4_quantize_device(_ptr(dBT), _ptr(dDT), ctypes.byref(op), flags, _stream()))
+
+
+def q4_pack_device(d_codes, d_scales, d_zeros, dDT, op):
+    """uint8[W][N] codes, float32[groups][N] scales, uint8[groups][N] zero points (or None) -> the operand's buffers."""
+    W = op.K // max(op.m, 1) * op.n
+    groups = -(-W // max(op.group, 1))
+    _need("q4_pack_device", d_codes=(d_codes, W * op.N), d_scales=(d_scales, groups * op.N), d_zeros=(d_zeros, groups * op.N),
+          dDT=(dDT, W * (op.N // 32)))
+    _check("nmspmm_q4_pack_device",
+           lib().nmspmm_q4_pack_device(_ptr(d_codes), _ptr(d_scales), _ptr(d_zeros), _ptr(dDT), ctypes.byref(op), _stream()))
+
+
+def q4_expand_device(op, dB):
+    _need("q4_expand_device", dB=(dB, op.K * op.N))
+    _check("nmspmm_q4_expand_device", lib().nmspmm_q4_expand_device(ctypes.byref(op), _ptr(dB), _stream()))
+
+
+def q4_linear(op, x, y, M, type, ldx=None, ldy=None):
+    """y [M, N] = x [M, K] times the operand plus its bias; rows ldx and ldy elements apart."""
+    ldx, ldy = op.K if ldx is None else ldx, op.N if ldy is None else ldy
+    if M > 0:
+        _need("q4_linear", x=(x, (M - 1) * ldx + op.K), y=(y, (M - 1) * ldy + op.N))
+    _check("nmspmm_q4_linear", lib().nmspmm_q4_linear(ctypes.byref(op), _ptr(x), ldx, _ptr(y), ldy, M, type, _stream()))
 
 
 # ---- host-pointer forms: arguments are C-contiguous numpy int32 arrays, updated in place ----------

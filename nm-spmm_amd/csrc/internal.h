@@ -552,5 +552,39 @@ hipError_t launch_decompress(const float* BT, const int32_t* DT, float* B, int K
 // dst[c * dst_ld + r] = src[r * cols + c] for a rows x cols row-major src (transpose.hip).
 hipError_t launch_transpose(const float* src, float* dst, int rows, int cols, int dst_ld, hipStream_t stream);
 
+// ---- operands in 4 bits (q4.hip, q4_linear.hip) ------------------------------------------------------
+
+// An operand of W kept rows (K dense ones) and N columns, already validated.
+struct Q4Shape {
+    int K, N, W;
+    int n, m;     // n kept rows in every window of m; 1, 1: dense
+    int group;    // kept rows that share a scale: 32, 64 or 128
+    int blocks;   // ceil(W / 128)
+    int tiles;    // 16-column tiles, an even number
+    int span;     // dense rows that 32 kept rows span: 32 m / n
+};
+
+enum ElementType { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+struct Q4LinearArgs {
+    const void* x;              // M rows of K elements, ldx elements apart
+    const uint32_t* codes;
+    const uint32_t* meta;
+    const uint8_t* rows;        // nullptr: dense
+    const float* bias;          // N or nullptr
+    void* y;                    // M rows of N elements of x's type, ldy elements apart
+    size_t ldx, ldy;
+    int M;
+    Q4Shape p;
+    hipStream_t stream;
+};
+
+hipError_t launch_q4_pack(const float* values, const uint8_t* given, const float* scales, const uint8_t* zeros,
+                          const int32_t* rows, const Q4Shape& p, bool asymmetric, uint32_t* codes, uint32_t* meta,
+                          uint8_t* row_offsets, hipStream_t stream);
+hipError_t launch_q4_expand(const uint32_t* codes, const uint32_t* meta, const uint8_t* row_offsets, const Q4Shape& p,
+                            float* B, hipStream_t stream);
+hipError_t launch_q4_linear(const Q4LinearArgs& a, ElementType type);
+
 } // namespace nmspmm
 #endif
