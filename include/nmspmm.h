@@ -379,6 +379,53 @@ typedef enum nmspmm_type { NMSPMM_F32 = 0, NMSPMM_BF16 = 1, NMSPMM_F16 = 2 } nms
 int nmspmm_q4_linear(const nmspmm_q4_operand* op, const void* x, long long ldx, void* y,
                      long long ldy, int M, int type, void* stream);
 
+/* ---- the norms around a block -------------------------------------------------------------- */
+
+/* No counterpart in the reference.  What stands between the compressed layers of one block of a model and
+ * those of the next, in one pass over the rows:
+ *     after = post(branch) * post_weight + post_bias
+ *     sum   = residual * scale + after * gate
+ *     out   = pre(sum) * pre_weight + pre_bias            (of the unrounded sum)
+ * post and pre: the RMS norm v / sqrt(mean(v^2) + eps), the Layer norm (v - mean(v)) / sqrt(var(v) + eps) of
+ * a row, or none.  Rows of `features` elements (1 to 16384), the leading dimensions in elements; below 2^31 rows.
+ * branch NULL: the first norm of a model, sum is the residual and is not written.  out NULL: the last sum.
+ * branch and out are of `type`; residual and sum of `residual_type`, the same or NMSPMM_F32.
+ * gate: [rows / gate_rows][features], each of its rows for gate_rows consecutive rows (all rows: one gate per
+ * feature; a sample's rows: one per sample; 1: one per element); scale: [features], where it is NULL the number
+ * `factor`; weights and biases: [features], weight_offset is added to both weights.  Each of these NULL: there is
+ * none; each has a type of its own.  stats: NULL, or float[rows][4] that the backward pass needs (16-byte aligned).
+ * All arithmetic is fp32, with one rounding of each result.  sum may be the residual's memory and out the
+ * branch's (with the same leading dimension).  16-byte aligned rows of whole groups of 8 elements are read
+ * and written 16 bytes at a time, anything else element by element. */
+typedef enum nmspmm_norm { NMSPMM_NORM_NONE = 0, NMSPMM_NORM_RMS = 1, NMSPMM_NORM_LAYER = 2 } nmspmm_norm;
+typedef struct nmspmm_block_norm {
+    long long rows, gate_rows, ld_residual, ld_branch, ld_sum, ld_out;
+    const void *residual, *branch;
+    void *sum, *out;
+    float* stats;
+    const void *gate, *scale, *post_weight, *post_bias, *pre_weight, *pre_bias;
+    int gate_type, scale_type, post_weight_type, post_bias_type, pre_weight_type, pre_bias_type;
+    int features, type, residual_type;
+    int post, pre; /* nmspmm_norm */
+    float factor, eps, weight_offset;
+} nmspmm_block_norm;
+int nmspmm_block_norm_forward(const nmspmm_block_norm* b, void* stream);
+
+/* The gradients: `b` as in the forward call, with the stats that it wrote (sum is not read, of out only whether
+ * it is NULL).  sum and out: the gradients that arrived, of their types, NULL for zero.  The others are written,
+ * of the types of what they belong to, where they are not NULL; sums over rows are taken in fp32 in a fixed order,
+ * so results repeat bit for bit.  rows >= 1. */
+typedef struct nmspmm_block_norm_grads {
+    long long ld_sum, ld_out, ld_residual, ld_branch;
+    const void *sum, *out;
+    void *residual, *branch;
+    void *gate, *scale, *post_weight, *post_bias, *pre_weight, *pre_bias;
+} nmspmm_block_norm_grads;
+/* Bytes of workspace of the backward call (gate_rows = rows where there is no gate); 0 for invalid arguments. */
+size_t nmspmm_block_norm_workspace_bytes(long long rows, long long gate_rows, int features);
+int nmspmm_block_norm_backward(const nmspmm_block_norm* b, const nmspmm_block_norm_grads* grads,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
 /* Frees what the library keeps per device: the cached split-K workspaces and the staging buffer
  * of the host-pointer preprocessing forms; forgets every attached row list. */
 int nmspmm_release(void);

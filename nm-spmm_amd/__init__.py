@@ -7,6 +7,7 @@ every call raises.
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libnmspmm.so")
@@ -33,6 +34,14 @@ class Q4Operand(ctypes.Structure):
     _fields_ = [("codes", ctypes.c_void_p), ("meta", ctypes.c_void_p), ("row_offsets", ctypes.c_void_p),
                 ("bias", ctypes.c_void_p), ("K", ctypes.c_int), ("N", ctypes.c_int), ("n", ctypes.c_int), ("m", ctypes.c_int),
                 ("group", ctypes.c_int)]
+
+
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2  # nmspmm_norm
+
+# nmspmm_block_norm and nmspmm_block_norm_grads as packed bytes, pointers as integers (0: NULL), fields in the
+# header's order: packing takes a tenth of what filling a ctypes.Structure of this many fields does
+BLOCK_NORM = struct.Struct("6q11P11i3f")
+BLOCK_NORM_GRADS = struct.Struct("4q10P")
 
 
 class NmSpmmError(RuntimeError):
@@ -102,6 +111,11 @@ def lib():
         L.nmspmm_q4_pack_device.argtypes = [c_void_p] * 4 + [op, c_void_p]
         L.nmspmm_q4_expand_device.argtypes = [op, c_void_p, c_void_p]
         L.nmspmm_q4_linear.argtypes = [op, c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p]
+        # (the two structs of the norms are packed bytes: BLOCK_NORM, BLOCK_NORM_GRADS)
+        L.nmspmm_block_norm_forward.argtypes = [ctypes.c_char_p, c_void_p]
+        L.nmspmm_block_norm_backward.argtypes = [ctypes.c_char_p, ctypes.c_char_p, c_void_p, c_size_t, c_void_p]
+        L.nmspmm_block_norm_workspace_bytes.restype = c_size_t
+        L.nmspmm_block_norm_workspace_bytes.argtypes = [ctypes.c_longlong, ctypes.c_longlong, c_int]
         L.nmspmm_release.restype = c_int
         _lib = L
     return _lib

@@ -1,0 +1,690 @@
+// What stands between two blocks of a model, in one pass over the rows:
+//     after = post(branch) w_post + b_post         (post: the RMS or the Layer norm of a row, or nothing)
+//     sum   = residual * scale + after * gate
+//     out   = pre(sum) w_pre + b_pre
+// and its gradients.  With v^ = (v - mean) / deviation (mean 0 for the RMS norm) and D features,
+//     d_sum'  = d_sum + (g - v^ mean(g v^) - mean(g)) / deviation,  g = d_out w_pre, v^ of sum (mean(g): Layer norm only)
+//     d_residual = d_sum' scale;  d_branch: the same formula once more with g = d_sum' gate w_post, v^ of branch;
+// the gradients of weights, biases, scale and gate are sums over rows of what stands next to them.
+// HBM-bound: forward reads residual and branch and writes sum and out, once each; backward reads residual,
+// branch, d_sum and d_out and writes d_residual and d_branch (sum is formed again: cheaper than to read its
+// rounded value, and exact).  A row stays in the registers of its threads, 8 or 16 elements each; statistics
+// and sums are fp32.  A thread keeps its columns' weights, and in the backward pass its columns' sums over
+// rows, in registers while it walks through a contiguous range of rows; the ranges' sums go to the workspace and
+// a second kernel adds them up in order, so that gradients repeat bit for bit.
+#include "internal.h"
+
+namespace nmspmm {
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxThreads = 1024;
+
+__device__ inline float from_bits16(uint32_t bits, int type)
+{
+    if (type == kBF16)
+        return __uint_as_float(bits << 16);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
+__device__ inline uint32_t to_bits16(float v, int type)
+{
+    if (type == kBF16)
+        return __builtin_bit_cast(uint16_t, (__bf16)v);
+    return __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+
+// The columns of a thread: VEC: 8 consecutive ones, `stride` threads times 8 between its groups of eight; otherwise single
+// ones, `stride` apart.
+template <bool VEC>
+__device__ inline int column_of(int t, int stride, int v, int e)
+{
+    return VEC ? (t + v * stride) * 8 + e : t + (v * 8 + e) * stride;
+}
+
+// Eight elements as they lie in memory: loads of several tensors can be under way before the first is unpacked.
+struct Raw {
+    u32x4 a, b;
+};
+template <bool VEC>
+__device__ inline Raw load_raw(const void* p, int type, size_t row, int t, int stride, int v, int D)
+{
+    Raw r = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+    if (VEC) {
+        const int c = column_of<true>(t, stride, v, 0);
+        if (c < D) {
+            if (type == kF32) {
+                const u32x4* const q = reinterpret_cast<const u32x4*>(static_cast<const float*>(p) + row + c);
+                r.a = q[0];
+                r.b = q[1];
+            } else
+                r.a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + row + c);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = column_of<false>(t, stride, v, e);
+            uint32_t x = 0;
+            if (c < D)
+                x = type == kF32 ? static_cast<const uint32_t*>(p)[row + c] : static_cast<const uint16_t*>(p)[row + c];
+            if (e < 4)
+                r.a[e] = x;
+            else
+                r.b[e - 4] = x;
+        }
+    }
+    return r;
+}
+template <bool VEC>
+__device__ inline void unpack(const Raw& r, int type, float* out)
+{
+    if (type == kF32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            out[e] = __uint_as_float(e < 4 ? r.a[e & 3] : r.b[e & 3]);
+    } else if (VEC) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            out[e] = from_bits16(e & 1 ? r.a[e >> 1] >> 16 : r.a[e >> 1] & 0xffffu, type);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            out[e] = from_bits16(e < 4 ? r.a[e & 3] : r.b[e & 3], type);
+    }
+}
+template <bool VEC>
+__device__ inline void store8(void* p, int type, size_t row, int t, int stride, int v, int D, const float* x)
+{
+    if (VEC) {
+        const int c = column_of<true>(t, stride, v, 0);
+        if (c >= D)
+            return;
+        if (type == kF32) {
+            u32x4* const q = reinterpret_cast<u32x4*>(static_cast<float*>(p) + row + c);
+            q[0] = u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+            q[1] = u32x4{__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])};
+        } else {
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[e] = to_bits16(x[2 * e], type) | to_bits16(x[2 * e + 1], type) << 16;
+            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + row + c) = w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int c = column_of<false>(t, stride, v, e);
+            if (c >= D)
+                continue;
+            if (type == kF32)
+                static_cast<float*>(p)[row + c] = x[e];
+            else
+                static_cast<uint16_t*>(p)[row + c] = (uint16_t)to_bits16(x[e], type);
+        }
+    }
+}
+
+// Sums over the threads of a row: a wave, or the workgroup's waves through LDS (two halves used in turn: one barrier a sum).
+struct RowSum {
+    float (*slots)[2][kMaxThreads / 64];
+    int half, waves;
+    __device__ void operator()(float& a, float& b)
+    {
+#pragma unroll
+        for (int mask = 1; mask < 64; mask <<= 1) {
+            a += __shfl_xor(a, mask, 64);
+            b += __shfl_xor(b, mask, 64);
+        }
+        if (waves == 1)
+            return;
+        if ((threadIdx.x & 63) == 0) {
+            slots[half][0][threadIdx.x >> 6] = a;
+            slots[half][1][threadIdx.x >> 6] = b;
+        }
+        __syncthreads();
+        a = b = 0.0f;
+        for (int w = 0; w < waves; ++w) {
+            a += slots[half][0][w];
+            b += slots[half][1][w];
+        }
+        half ^= 1;
+    }
+};
+
+// Mean (Layer norm) and 1 / deviation of the row whose elements the threads hold (zeros beyond D); v becomes v^.
+template <int E>
+__device__ inline void standardize(float* v, const bool* in, int kind, float inv_d, float eps, RowSum& sum, float& mean, float& inv)
+{
+    float a = 0.0f, b = 0.0f;
+    mean = 0.0f;
+    if (kind == kLayerNorm) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            a += v[e];
+        sum(a, b);
+        mean = a * inv_d;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            v[e] = in[e] ? v[e] - mean : 0.0f;
+        a = b = 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        a = fmaf(v[e], v[e], a);
+    sum(a, b);
+    inv = 1.0f / sqrtf(a * inv_d + eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        v[e] *= inv;
+}
+
+// The thread's columns of the parameters (1, 0 or the plain factor where there is none).
+template <bool VEC, int NV>
+struct Columns {
+    float post_w[NV * 8], post_b[NV * 8], scale[NV * 8], pre_w[NV * 8], pre_b[NV * 8], gate[NV * 8];
+
+    // everything that does not change from row to row: all loads first, then their values
+    __device__ void load(const BlockNormArgs& a, size_t gate_row, bool with_gate, int t, int stride)
+    {
+        Raw pw[NV], pb[NV], sc[NV], nw[NV], nb[NV], g[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if (a.post_weight.data)
+                pw[v] = load_raw<VEC>(a.post_weight.data, a.post_weight.type, 0, t, stride, v, a.D);
+            if (a.post_bias.data)
+                pb[v] = load_raw<VEC>(a.post_bias.data, a.post_bias.type, 0, t, stride, v, a.D);
+            if (a.scale.data)
+                sc[v] = load_raw<VEC>(a.scale.data, a.scale.type, 0, t, stride, v, a.D);
+            if (a.pre_weight.data)
+                nw[v] = load_raw<VEC>(a.pre_weight.data, a.pre_weight.type, 0, t, stride, v, a.D);
+            if (a.pre_bias.data)
+                nb[v] = load_raw<VEC>(a.pre_bias.data, a.pre_bias.type, 0, t, stride, v, a.D);
+            if (with_gate)
+                g[v] = load_raw<VEC>(a.gate.data, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D);
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            value(a.post_weight, pw[v], 1.0f, a.weight_offset, post_w + v * 8);
+            value(a.post_bias, pb[v], 0.0f, 0.0f, post_b + v * 8);
+            value(a.scale, sc[v], a.factor, 0.0f, scale + v * 8);
+            value(a.pre_weight, nw[v], 1.0f, a.weight_offset, pre_w + v * 8);
+            value(a.pre_bias, nb[v], 0.0f, 0.0f, pre_b + v * 8);
+            if (with_gate)
+                unpack<VEC>(g[v], a.gate.type, gate + v * 8);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    gate[v * 8 + e] = 1.0f;
+        }
+    }
+    __device__ void load_gate(const BlockNormArgs& a, size_t gate_row, int t, int stride)
+    {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            unpack<VEC>(load_raw<VEC>(a.gate.data, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D), a.gate.type, gate + v * 8);
+    }
+
+private:
+    __device__ static void value(const BlockNormVec& p, const Raw& r, float missing, float offset, float* out)
+    {
+        if (p.data) {
+            unpack<VEC>(r, p.type, out);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                out[e] += offset;
+        } else
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                out[e] = missing;
+    }
+};
+
+// ---- forward ------------------------------------------------------------------------------------------
+
+template <ElementType T, ElementType R, bool VEC, int NV>
+__global__ void __launch_bounds__(kMaxThreads)
+block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
+{
+    __shared__ float slots[2][2][kMaxThreads / 64];
+    constexpr int E = NV * 8;
+    const int t = threadIdx.x % row_threads;
+    const int walker = blockIdx.x * (blockDim.x / row_threads) + threadIdx.x / row_threads;
+    if (walker >= walkers)      // whole waves, and only where a row is one wave: no barrier is missed
+        return;
+    const size_t begin = (size_t)walker * a.rows / walkers, end = (size_t)(walker + 1) * a.rows / walkers;
+    const int stride = row_threads;
+    const float inv_d = 1.0f / (float)a.D;
+    RowSum sum = {slots, 0, row_threads / 64};
+    bool in[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        in[e] = column_of<VEC>(t, stride, e / 8, e % 8) < a.D;
+
+    const bool branch = a.branch != nullptr, gated = branch && a.gate.data != nullptr;
+    Raw rr[NV], yr[NV];
+    auto load = [&](size_t row) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            rr[v] = load_raw<VEC>(a.residual, R, row * a.ld_residual, t, stride, v, a.D);
+            if (branch)
+                yr[v] = load_raw<VEC>(a.branch, T, row * a.ld_branch, t, stride, v, a.D);
+        }
+    };
+    if (begin < end)
+        load(begin);
+    Columns<VEC, NV> p;
+    size_t gate_row = begin / a.gate_rows;
+    p.load(a, gate_row, gated, t, stride);
+
+    for (size_t row = begin; row < end; ++row) {
+        float s[E], mean, inv;
+        float post_mean = 0.0f, post_inv = 1.0f, pre_mean = 0.0f, pre_inv = 1.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            unpack<VEC>(rr[v], R, s + v * 8);
+        if (branch) {
+            float y[E];
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                unpack<VEC>(yr[v], T, y + v * 8);
+            if (gated && row / a.gate_rows != gate_row) {
+                gate_row = row / a.gate_rows;
+                p.load_gate(a, gate_row, t, stride);
+            }
+            if (row + 1 < end)
+                load(row + 1);
+            if (a.post != kNoNorm) {
+                standardize<E>(y, in, a.post, inv_d, a.eps, sum, mean, inv);
+                post_mean = mean;
+                post_inv = inv;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    y[e] = fmaf(y[e], p.post_w[e], p.post_b[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                s[e] = fmaf(s[e], p.scale[e], y[e] * p.gate[e]);
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                store8<VEC>(a.sum, R, row * a.ld_sum, t, stride, v, a.D, s + v * 8);
+        } else if (row + 1 < end)
+            load(row + 1);
+        if (a.out) {
+            // columns beyond D: s may hold a bias there, it must not count
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                s[e] = in[e] ? s[e] : 0.0f;
+            if (a.pre != kNoNorm) {
+                standardize<E>(s, in, a.pre, inv_d, a.eps, sum, mean, inv);
+                pre_mean = mean;
+                pre_inv = inv;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    s[e] = fmaf(s[e], p.pre_w[e], p.pre_b[e]);
+            }
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                store8<VEC>(a.out, T, row * a.ld_out, t, stride, v, a.D, s + v * 8);
+        }
+        if (a.stats && t == 0)
+            *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(post_mean, post_inv, pre_mean, pre_inv);
+    }
+}
+
+// ---- backward -----------------------------------------------------------------------------------------
+
+template <ElementType T, ElementType R, bool VEC, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, int walkers, int per_gate, int gates_each)
+{
+    __shared__ float slots[2][2][kMaxThreads / 64];
+    constexpr int E = NV * 8;
+    const int t = threadIdx.x % row_threads;
+    const int walker = blockIdx.x * (blockDim.x / row_threads) + threadIdx.x / row_threads;
+    if (walker >= walkers)
+        return;
+    // a walker's rows: part `walker % per_gate` of a gate's rows, or those of `gates_each` whole gates
+    const size_t gates = (a.rows + a.gate_rows - 1) / a.gate_rows;
+    size_t begin, end;
+    if (per_gate > 1) {
+        const size_t g = walker / per_gate, part = walker % per_gate;
+        begin = g * a.gate_rows + part * a.gate_rows / per_gate;
+        end = g * a.gate_rows + (part + 1) * a.gate_rows / per_gate;
+    } else {
+        begin = (size_t)walker * gates_each * a.gate_rows;
+        end = min(begin + (size_t)gates_each * a.gate_rows, gates * a.gate_rows);
+    }
+    const int stride = row_threads;
+    const float inv_d = 1.0f / (float)a.D;
+    RowSum sum = {slots, 0, row_threads / 64};
+    const bool branch = a.branch != nullptr, gated = branch && a.gate.data != nullptr;
+
+    Columns<VEC, NV> p;
+    size_t gate_row = begin / a.gate_rows;
+    p.load(a, gate_row, gated, t, stride);
+    float sum_post_w[E], sum_post_b[E], sum_scale[E], sum_pre_w[E], sum_pre_b[E], sum_gate[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        sum_post_w[e] = sum_post_b[e] = sum_scale[e] = sum_pre_w[e] = sum_pre_b[e] = sum_gate[e] = 0.0f;
+
+    for (size_t row = begin; row < end; ++row) {
+        Raw rr[NV], yr[NV], gs[NV], go[NV];
+        const float4 st = *reinterpret_cast<const float4*>(a.stats + row * 4);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            rr[v] = load_raw<VEC>(a.residual, R, row * a.ld_residual, t, stride, v, a.D);
+            if (branch)
+                yr[v] = load_raw<VEC>(a.branch, T, row * a.ld_branch, t, stride, v, a.D);
+            if (d.sum)
+                gs[v] = load_raw<VEC>(d.sum, R, row * d.ld_sum, t, stride, v, a.D);
+            if (d.out)
+                go[v] = load_raw<VEC>(d.out, T, row * d.ld_out, t, stride, v, a.D);
+        }
+        if (gated && row / a.gate_rows != gate_row) {
+            if (d.gate && per_gate == 1)
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+                    store8<VEC>(d.gate, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D, sum_gate + v * 8);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                sum_gate[e] = 0.0f;
+            gate_row = row / a.gate_rows;
+            p.load_gate(a, gate_row, t, stride);
+        }
+        float r[E], yn[E], s[E], ds[E];
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            unpack<VEC>(rr[v], R, r + v * 8);
+        if (branch) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                unpack<VEC>(yr[v], T, yn + v * 8);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                yn[e] = (yn[e] - st.x) * st.y;      // mean 0 and 1 / deviation 1 where there is no norm
+                s[e] = fmaf(r[e], p.scale[e], fmaf(yn[e], p.post_w[e], p.post_b[e]) * p.gate[e]);
+            }
+        } else
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                s[e] = r[e];
+        if (d.sum)
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                unpack<VEC>(gs[v], R, ds + v * 8);
+        else
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                ds[e] = 0.0f;
+        if (d.out) {
+            float g[E];
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                unpack<VEC>(go[v], T, g + v * 8);   // zeros beyond D
+            float with = 0.0f, plain = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                s[e] = (s[e] - st.z) * st.w;
+                sum_pre_w[e] = fmaf(g[e], s[e], sum_pre_w[e]);
+                sum_pre_b[e] += g[e];
+                g[e] *= p.pre_w[e];
+                with = fmaf(g[e], s[e], with);
+                plain += g[e];
+            }
+            if (a.pre != kNoNorm) {
+                sum(with, plain);
+                with *= inv_d;
+                plain = a.pre == kLayerNorm ? plain * inv_d : 0.0f;
+            } else
+                with = plain = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                ds[e] = fmaf(st.w, g[e] - fmaf(s[e], with, plain), ds[e]);
+        }
+        if (!branch) {
+            if (d.residual)
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+                    store8<VEC>(d.residual, R, row * d.ld_residual, t, stride, v, a.D, ds + v * 8);
+            continue;
+        }
+        float with = 0.0f, plain = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (column_of<VEC>(t, stride, e / 8, e % 8) >= a.D)
+                ds[e] = 0.0f;
+            sum_scale[e] = fmaf(ds[e], r[e], sum_scale[e]);
+            sum_gate[e] = fmaf(ds[e], fmaf(yn[e], p.post_w[e], p.post_b[e]), sum_gate[e]);
+            r[e] = ds[e] * p.scale[e];
+            ds[e] *= p.gate[e];
+            sum_post_w[e] = fmaf(ds[e], yn[e], sum_post_w[e]);
+            sum_post_b[e] += ds[e];
+            ds[e] *= p.post_w[e];
+            with = fmaf(ds[e], yn[e], with);
+            plain += ds[e];
+        }
+        if (d.residual)
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                store8<VEC>(d.residual, R, row * d.ld_residual, t, stride, v, a.D, r + v * 8);
+        if (a.post != kNoNorm) {
+            sum(with, plain);
+            with *= inv_d;
+            plain = a.post == kLayerNorm ? plain * inv_d : 0.0f;
+        } else
+            with = plain = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            ds[e] = st.y * (ds[e] - fmaf(yn[e], with, plain));
+        if (d.branch)
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                store8<VEC>(d.branch, T, row * d.ld_branch, t, stride, v, a.D, ds + v * 8);
+    }
+
+    if (gated && d.gate && per_gate == 1 && begin < end)
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            store8<VEC>(d.gate, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D, sum_gate + v * 8);
+    // the walker's sums: [parameter][walker][column]
+    auto leave = [&](int slot, const float* x) {
+        if (slot >= 0)
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                store8<VEC>(d.partial, kF32, ((size_t)slot * walkers + walker) * a.D, t, stride, v, a.D, x + v * 8);
+    };
+    leave(d.slot_post_weight, sum_post_w);
+    leave(d.slot_post_bias, sum_post_b);
+    leave(d.slot_scale, sum_scale);
+    leave(d.slot_pre_weight, sum_pre_w);
+    leave(d.slot_pre_bias, sum_pre_b);
+    leave(d.slot_gate, sum_gate);
+}
+
+// Adds the walkers' sums up in order: 64 columns per workgroup, its 16 waves take the walkers in turn.
+struct FinishArgs {
+    const float* partial;
+    void* out[6];
+    int type[6], slot[6];
+    int outputs;        // of a whole column each; the gate, if it is here, is the last
+    int gate;           // its place among them, -1 if it is not here
+    int gates, per_gate;
+    int walkers, D;
+};
+__global__ void __launch_bounds__(1024)
+block_norm_finish_kernel(FinishArgs f)
+{
+    __shared__ float part[16][64];
+    const int x = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int col = blockIdx.x * 64 + x;
+    int o = blockIdx.y, g = 0, first = 0, count = f.walkers;
+    if (f.gate >= 0 && o >= f.gate) {
+        g = o - f.gate;
+        o = f.gate;
+        first = g * f.per_gate;
+        count = f.per_gate;
+    }
+    float sum = 0.0f;
+    if (col < f.D) {
+        const float* const p = f.partial + ((size_t)f.slot[o] * f.walkers + first) * f.D + col;
+#pragma unroll 4
+        for (int i = w; i < count; i += 16)
+            sum += p[(size_t)i * f.D];
+    }
+    part[w][x] = sum;
+    __syncthreads();
+    if (w == 0 && col < f.D) {
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            sum += part[i][x];
+        const size_t at = (size_t)g * f.D + col;
+        if (f.type[o] == kF32)
+            static_cast<float*>(f.out[o])[at] = sum;
+        else
+            static_cast<uint16_t*>(f.out[o])[at] = (uint16_t)to_bits16(sum, f.type[o]);
+    }
+}
+
+// Threads of a row, in whole waves: 8 elements each up to 8192 features, 16 beyond.
+int row_threads_of(int D)
+{
+    const int each = D <= 8 * kMaxThreads ? 8 : 16;
+    return (((D + each - 1) / each) + 63) / 64 * 64;
+}
+
+bool vector_rows(const void* p, size_t ld, int D)
+{
+    return !p || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0 && D % 8 == 0);
+}
+
+bool vector_forward(const BlockNormArgs& a)
+{
+    const size_t D = a.D;
+    return vector_rows(a.residual, a.ld_residual, a.D) && vector_rows(a.branch, a.ld_branch, a.D) && vector_rows(a.sum, a.ld_sum, a.D) &&
+           vector_rows(a.out, a.ld_out, a.D) && vector_rows(a.gate.data, D, a.D) && vector_rows(a.scale.data, D, a.D) &&
+           vector_rows(a.post_weight.data, D, a.D) && vector_rows(a.post_bias.data, D, a.D) &&
+           vector_rows(a.pre_weight.data, D, a.D) && vector_rows(a.pre_bias.data, D, a.D);
+}
+
+template <ElementType T, ElementType R, bool VEC>
+void forward(const BlockNormArgs& a, hipStream_t stream)
+{
+    const int rt = row_threads_of(a.D), each = rt == 64 ? 4 : 1;
+    // as many walkers as the GPU holds waves of this many registers (16 a compute unit)
+    const size_t most = (size_t)machine().cus * 16 / (rt / 64);
+    const int walkers = (int)(a.rows < most ? a.rows : most);
+    const dim3 grid((walkers + each - 1) / each), block(rt * each);
+    if (a.D <= 8 * kMaxThreads)
+        block_norm_kernel<T, R, VEC, 1><<<grid, block, 0, stream>>>(a, rt, walkers);
+    else
+        block_norm_kernel<T, R, VEC, 2><<<grid, block, 0, stream>>>(a, rt, walkers);
+}
+
+template <ElementType T, ElementType R, bool VEC>
+void backward(const BlockNormArgs& a, const BlockNormGrads& d, const BlockNormWalk& w, hipStream_t stream)
+{
+    const int rt = row_threads_of(a.D), each = rt == 64 ? 4 : 1;
+    const dim3 grid((w.walkers + each - 1) / each), block(rt * each);
+    if (a.D <= 4096)
+        block_norm_backward_kernel<T, R, VEC, 1, 512><<<grid, block, 0, stream>>>(a, d, rt, w.walkers, w.per_gate, w.gates_each);
+    else if (a.D <= 8 * kMaxThreads)
+        block_norm_backward_kernel<T, R, VEC, 1, 1024><<<grid, block, 0, stream>>>(a, d, rt, w.walkers, w.per_gate, w.gates_each);
+    else
+        block_norm_backward_kernel<T, R, VEC, 2, 1024><<<grid, block, 0, stream>>>(a, d, rt, w.walkers, w.per_gate, w.gates_each);
+}
+
+} // namespace
+
+hipError_t launch_block_norm(const BlockNormArgs& a, int type, int residual_type, hipStream_t stream)
+{
+    const bool vec = vector_forward(a);
+#define NMSPMM_TYPES(T, R) (vec ? forward<T, R, true>(a, stream) : forward<T, R, false>(a, stream))
+    if (type == kF32)
+        NMSPMM_TYPES(kF32, kF32);
+    else if (type == kBF16)
+        residual_type == kF32 ? NMSPMM_TYPES(kBF16, kF32) : NMSPMM_TYPES(kBF16, kBF16);
+    else
+        residual_type == kF32 ? NMSPMM_TYPES(kF16, kF32) : NMSPMM_TYPES(kF16, kF16);
+#undef NMSPMM_TYPES
+    return hipGetLastError();
+}
+
+// How the backward pass cuts the rows: about two workgroups per compute unit, at least four rows each, and no
+// walker with a part of a gate's rows beside rows of another gate.
+BlockNormWalk block_norm_walk(long long rows, long long gate_rows, int D)
+{
+    const int waves = row_threads_of(D) / 64;
+    const long long most = (long long)machine().cus * 16 / (waves < 8 ? waves : 8);
+    long long rows_each = (rows + most - 1) / most;
+    if (rows_each < 4)
+        rows_each = 4;
+    const long long gates = (rows + gate_rows - 1) / gate_rows;
+    BlockNormWalk w = {0, 1, 1};
+    if (gate_rows > rows_each) {
+        w.per_gate = (int)((gate_rows + rows_each - 1) / rows_each);
+        w.walkers = (int)(gates * w.per_gate);
+    } else {
+        w.gates_each = (int)(rows_each / gate_rows);
+        w.walkers = (int)((gates + w.gates_each - 1) / w.gates_each);
+    }
+    return w;
+}
+
+hipError_t launch_block_norm_backward(const BlockNormArgs& a, const BlockNormGrads& given, int type, int residual_type,
+                                      hipStream_t stream)
+{
+    BlockNormGrads d = given;
+    const BlockNormWalk w = block_norm_walk(a.rows, a.gate_rows, a.D);
+    FinishArgs f = {};
+    f.partial = d.partial;
+    f.gate = -1;
+    f.gates = 1;
+    f.walkers = w.walkers;
+    f.D = a.D;
+    int slots = 0;
+    auto column = [&](void* out, int out_type, int& slot) {
+        slot = -1;
+        if (!out)
+            return;
+        slot = slots;
+        f.out[slots] = out;
+        f.type[slots] = out_type;
+        f.slot[slots] = slots;
+        ++slots;
+    };
+    column(d.post_weight, a.post_weight.type, d.slot_post_weight);
+    column(d.post_bias, a.post_bias.type, d.slot_post_bias);
+    column(d.scale, a.scale.type, d.slot_scale);
+    column(d.pre_weight, a.pre_weight.type, d.slot_pre_weight);
+    column(d.pre_bias, a.pre_bias.type, d.slot_pre_bias);
+    d.slot_gate = -1;
+    int outputs = slots;
+    if (d.gate && w.per_gate > 1) {
+        f.gate = slots;
+        f.gates = (int)((a.rows + a.gate_rows - 1) / a.gate_rows);
+        f.per_gate = w.per_gate;
+        column(d.gate, a.gate.type, d.slot_gate);
+        outputs += f.gates;
+    }
+    const size_t D = a.D;
+    const bool vec = vector_forward(a) && vector_rows(d.sum, d.ld_sum, a.D) && vector_rows(d.out, d.ld_out, a.D) &&
+                     vector_rows(d.residual, d.ld_residual, a.D) && vector_rows(d.branch, d.ld_branch, a.D) &&
+                     vector_rows(d.gate, D, a.D);
+    if (a.rows > 0) {
+#define NMSPMM_TYPES(T, R) (vec ? backward<T, R, true>(a, d, w, stream) : backward<T, R, false>(a, d, w, stream))
+        if (type == kF32)
+            NMSPMM_TYPES(kF32, kF32);
+        else if (type == kBF16)
+            residual_type == kF32 ? NMSPMM_TYPES(kBF16, kF32) : NMSPMM_TYPES(kBF16, kBF16);
+        else
+            residual_type == kF32 ? NMSPMM_TYPES(kF16, kF32) : NMSPMM_TYPES(kF16, kF16);
+#undef NMSPMM_TYPES
+    }
+    if (outputs > 0)
+        block_norm_finish_kernel<<<dim3((a.D + 63) / 64, outputs), 1024, 0, stream>>>(f);
+    return hipGetLastError();
+}
+
+} // namespace nmspmm

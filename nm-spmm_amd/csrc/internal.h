@@ -586,5 +586,50 @@ hipError_t launch_q4_expand(const uint32_t* codes, const uint32_t* meta, const u
                             float* B, hipStream_t stream);
 hipError_t launch_q4_linear(const Q4LinearArgs& a, ElementType type);
 
+// ---- the norms around a block (block_norm.hip) ---------------------------------------------------------
+
+enum NormKind { kNoNorm = 0, kRmsNorm = 1, kLayerNorm = 2 };
+
+struct BlockNormVec {
+    const void* data;   // nullptr: there is none
+    int type;           // ElementType
+};
+
+struct BlockNormArgs {
+    size_t rows;
+    int D;
+    const void* residual;       // rows `ld_` elements apart, here and below
+    const void* branch;         // nullptr: sum is the residual and is not written
+    void* sum;
+    void* out;                  // nullptr: not wanted
+    float* stats;               // [rows][4]: mean and 1 / deviation of branch, then of sum; nullptr: not wanted
+    size_t ld_residual, ld_branch, ld_sum, ld_out;
+    size_t gate_rows;           // consecutive rows that share a row of the gate
+    BlockNormVec gate, scale, post_weight, post_bias, pre_weight, pre_bias;
+    float factor;               // where there is no scale
+    float eps, weight_offset;
+    int post, pre;              // NormKind
+};
+
+struct BlockNormGrads {
+    const void* sum;            // gradients that came in; nullptr: zero
+    const void* out;
+    void* residual;             // gradients to be written; nullptr: not wanted
+    void* branch;
+    size_t ld_sum, ld_out, ld_residual, ld_branch;
+    void *gate, *scale, *post_weight, *post_bias, *pre_weight, *pre_bias;   // of their parameters' types
+    float* partial;             // [parameter][walker][D]
+    int slot_gate, slot_scale, slot_post_weight, slot_post_bias, slot_pre_weight, slot_pre_bias;
+};
+
+struct BlockNormWalk {
+    int walkers, per_gate, gates_each;
+};
+BlockNormWalk block_norm_walk(long long rows, long long gate_rows, int D);
+
+hipError_t launch_block_norm(const BlockNormArgs& a, int type, int residual_type, hipStream_t stream);
+hipError_t launch_block_norm_backward(const BlockNormArgs& a, const BlockNormGrads& d, int type, int residual_type,
+                                      hipStream_t stream);
+
 } // namespace nmspmm
 #endif

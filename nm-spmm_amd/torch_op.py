@@ -10,7 +10,7 @@ The reference has no framework binding; its driver multiplies synthetic operands
 (tests/test_nmspmm.cu:72-97).  The sequence of calls here is that driver's, on real weights.
 """
 import importlib
-from typing import Optional
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -336,3 +336,288 @@ class NMQuantLinear(torch.nn.Module):
     def extra_repr(self):
         return "in_features=%d, out_features=%d, pattern=%d:%d, group=%d, bias=%s" % (
             self.in_features, self.out_features, self.n, self.m, self.group, self._buffers["bias"] is not None)
+
+
+# ---- the norms around a block -----------------------------------------------------------------------
+
+_NORMS = {None: _nm.NORM_NONE, "rms": _nm.NORM_RMS, "layer": _nm.NORM_LAYER}
+_PARAMS = ("gate", "residual_scale", "post_weight", "post_bias", "pre_weight", "pre_bias")
+
+
+def _as_rows(t, D):
+    """(t, elements between its rows): t itself where its leading dimensions can be walked as rows, else a copy."""
+    if t.is_contiguous():
+        return t, D
+    rows = t.reshape(-1, D)
+    if (D > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < D):
+        rows = rows.contiguous()
+    return rows, max(rows.stride(0), D)
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _pack_block_norm(residual, branch, total, out, stats, params, factor, post, pre, eps, weight_offset, gate_rows, dtype):
+    """The packed struct, and the tensors (possibly copies) whose memory it names."""
+    D = residual.shape[-1]
+    rows = residual.numel() // D
+    residual, ld_residual = _as_rows(residual, D)
+    ld_branch = D
+    if branch is not None:
+        branch, ld_branch = _as_rows(branch, D)
+    gate, scale, post_w, post_b, pre_w, pre_b = params = [p if p is None or p.is_contiguous() else p.contiguous() for p in params]
+    packed = _nm.BLOCK_NORM.pack(
+        rows, gate_rows, ld_residual, ld_branch, D, D, residual.data_ptr(), _at(branch), _at(total), _at(out), _at(stats),
+        _at(gate), _at(scale), _at(post_w), _at(post_b), _at(pre_w), _at(pre_b),
+        *[0 if p is None else _TYPES[p.dtype] for p in params],
+        D, _TYPES[dtype], _TYPES[residual.dtype], post, pre, factor, eps, weight_offset)
+    return packed, (residual, branch, params)
+
+
+def _block_norm_forward(residual, branch, params, factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out, want_stats):
+    """(sum or None, out or None, stats or None)."""
+    total = None if branch is None else residual.new_empty(residual.shape)
+    out = residual.new_empty(residual.shape, dtype=dtype) if want_out else None
+    stats = residual.new_empty((residual.numel() // residual.shape[-1], 4), dtype=torch.float32) if want_stats else None
+    if residual.numel() == 0:
+        return total, out, stats
+    packed, keep = _pack_block_norm(residual, branch, total, out, stats, params, factor, post, pre, eps, weight_offset, gate_rows, dtype)
+    device = residual.device
+    if device.index != torch.cuda.current_device():
+        with _guard(residual):
+            status = _nm.lib().nmspmm_block_norm_forward(packed, _on(device))
+    else:
+        status = _nm.lib().nmspmm_block_norm_forward(packed, _on(device))
+    if status != _nm.OK:
+        raise _nm.NmSpmmError("nmspmm_block_norm_forward", status)
+    return total, out, stats
+
+
+def _block_norm_backward(residual, branch, params, stats, grad_sum, grad_out, factor, post, pre, eps, weight_offset, gate_rows,
+                         dtype, want_out, needs):
+    """Gradients of (residual, branch, *params), None where `needs` is false or there is no such input."""
+    D = residual.shape[-1]
+    given = (residual, branch, *params)
+    if residual.numel() == 0:
+        return [torch.zeros_like(t) if need and t is not None else None for t, need in zip(given, needs)]
+    grads = [t.new_empty(t.shape) if need and t is not None else None for t, need in zip(given, needs)]
+    ld_sum = ld_out = D
+    if grad_sum is not None:
+        grad_sum, ld_sum = _as_rows(grad_sum, D)
+    if grad_out is not None:
+        grad_out, ld_out = _as_rows(grad_out, D)
+    # of the forward pass's results only whether there was an `out` counts: any address stands for it
+    total, out = (None if branch is None else residual), (stats if want_out else None)
+    packed, keep = _pack_block_norm(residual, branch, total, out, stats, params, factor, post, pre, eps, weight_offset, gate_rows, dtype)
+    want = _nm.BLOCK_NORM_GRADS.pack(ld_sum, ld_out, D, D, _at(grad_sum), _at(grad_out), *[_at(g) for g in grads])
+    with _guard(residual):
+        rows = residual.numel() // D
+        bytes_ = _nm.lib().nmspmm_block_norm_workspace_bytes(rows, gate_rows, D)
+        workspace = residual.new_empty(bytes_ // 4, dtype=torch.float32)
+        status = _nm.lib().nmspmm_block_norm_backward(packed, want, workspace.data_ptr(), bytes_, _on(residual.device))
+    if status != _nm.OK:
+        raise _nm.NmSpmmError("nmspmm_block_norm_backward", status)
+    return grads
+
+
+class _BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, residual, branch, gate, scale, post_w, post_b, pre_w, pre_b, conf):
+        factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out = conf
+        params = (gate, scale, post_w, post_b, pre_w, pre_b)
+        total, out, stats = _block_norm_forward(residual, branch, params, *conf, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(residual, branch, *params, stats)
+        ctx.conf = conf
+        # without a branch the sum is the residual, as an output of its own: its gradient comes to the same kernel
+        return residual.view_as(residual) if total is None else total, out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_sum, grad_out):
+        residual, branch, *params, stats = ctx.saved_tensors
+        if grad_sum is None and grad_out is None:
+            return (None,) * 9
+        return (*_block_norm_backward(residual, branch, params, stats, grad_sum, grad_out, *ctx.conf, ctx.needs_input_grad[:8]), None)
+
+
+# The same for tracing front ends: one node forward, one backward.  What is not wanted is an empty tensor.
+
+@torch.library.custom_op("nmspmm::block_norm", mutates_args=(), device_types="cuda")
+def _block_norm_op(residual: torch.Tensor, branch: Optional[torch.Tensor], gate: Optional[torch.Tensor], scale: Optional[torch.Tensor],
+                   post_weight: Optional[torch.Tensor], post_bias: Optional[torch.Tensor], pre_weight: Optional[torch.Tensor],
+                   pre_bias: Optional[torch.Tensor], factor: float, post: int, pre: int, eps: float, weight_offset: float,
+                   gate_rows: int, dtype: torch.dtype, want_out: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    total, out, stats = _block_norm_forward(residual, branch, (gate, scale, post_weight, post_bias, pre_weight, pre_bias), factor, post,
+                                            pre, eps, weight_offset, gate_rows, dtype, want_out, True)
+    nothing = lambda: residual.new_empty(0)  # noqa: E731
+    return nothing() if total is None else total, nothing() if out is None else out, stats
+
+
+@_block_norm_op.register_fake
+def _block_norm_fake(residual, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias, factor, post, pre, eps,
+                     weight_offset, gate_rows, dtype, want_out):
+    total = residual.new_empty(0 if branch is None else residual.shape)
+    out = residual.new_empty(residual.shape, dtype=dtype) if want_out else residual.new_empty(0)
+    return total, out, residual.new_empty((residual.numel() // residual.shape[-1], 4), dtype=torch.float32)
+
+
+@torch.library.custom_op("nmspmm::block_norm_backward", mutates_args=(), device_types="cuda")
+def _block_norm_backward_op(residual: torch.Tensor, branch: Optional[torch.Tensor], gate: Optional[torch.Tensor],
+                            scale: Optional[torch.Tensor], post_weight: Optional[torch.Tensor], post_bias: Optional[torch.Tensor],
+                            pre_weight: Optional[torch.Tensor], pre_bias: Optional[torch.Tensor], stats: torch.Tensor,
+                            grad_sum: Optional[torch.Tensor], grad_out: Optional[torch.Tensor], factor: float, post: int, pre: int,
+                            eps: float, weight_offset: float, gate_rows: int, dtype: torch.dtype, want_out: bool,
+                            needs: List[bool]) -> List[torch.Tensor]:
+    grads = _block_norm_backward(residual, branch, (gate, scale, post_weight, post_bias, pre_weight, pre_bias), stats, grad_sum, grad_out,
+                                 factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out, needs)
+    return [residual.new_empty(0) if g is None else g for g in grads]
+
+
+@_block_norm_backward_op.register_fake
+def _block_norm_backward_fake(residual, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias, stats, grad_sum, grad_out,
+                              factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out, needs):
+    given = (residual, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
+    return [t.new_empty(t.shape) if need and t is not None else residual.new_empty(0) for t, need in zip(given, needs)]
+
+
+def _block_norm_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:8], output[2])
+    ctx.conf = inputs[8:]
+    ctx.has_branch = inputs[1] is not None
+
+
+def _block_norm_gradients(ctx, grad_sum, grad_out, grad_stats):
+    *given, stats = ctx.saved_tensors
+    needs = list(ctx.needs_input_grad[:8])
+    if not ctx.has_branch:
+        grad_sum = None
+    if not ctx.conf[7]:
+        grad_out = None
+    if grad_sum is None and grad_out is None:
+        return (None,) * 16
+    grads = _block_norm_backward_op(*given, stats, grad_sum, grad_out, *ctx.conf, needs)
+    return (*[g if need and t is not None else None for g, need, t in zip(grads, needs, given)], *([None] * 8))
+
+
+_block_norm_op.register_autograd(_block_norm_gradients, setup_context=_block_norm_setup)
+
+
+def _gate_rows(gate, shape):
+    """(gate, consecutive rows that share one of its rows) for a gate that broadcasts against `shape`."""
+    D = shape[-1]
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    if gate.shape == (D,):
+        return gate, rows
+    if gate.dim() == len(shape) and gate.shape[-1] == D:
+        lead, each = 0, 1
+        while lead < len(shape) - 1 and gate.shape[lead] == shape[lead]:
+            lead += 1
+        for n in shape[lead:-1]:
+            each *= n
+        if all(n == 1 for n in gate.shape[lead:-1]):
+            return gate, each
+    return gate.expand(shape), 1
+
+
+def block_norm(residual, branch=None, *, gate=None, residual_scale=1.0, post=None, post_weight=None, post_bias=None, pre="rms",
+               pre_weight=None, pre_bias=None, eps=1e-6, weight_offset=0.0, dtype=None):
+    """The norm after a block, its gate, the scaled residual sum and the norm before the next block, in one launch:
+
+        after = post(branch) * post_weight + post_bias
+        sum   = residual * residual_scale + after * gate
+        out   = pre(sum) * pre_weight + pre_bias
+
+    and returns (sum, out).  residual [..., D] and branch of its shape, D up to 16384; post and pre are "rms", "layer" or None; without
+    a branch (the first norm of a model) sum is the residual; with pre None out is None.  gate broadcasts against
+    branch ([D], [batch, 1, D], a whole [batch, tokens, D], ...); residual_scale is a number or a tensor [D] (or of one element); weights and
+    biases are [D], weight_offset is added to the weights.  residual is float32 or of branch's type; `dtype` is out's type
+    (branch's where there is one, else residual's unless given).  All arithmetic is float32.  Differentiable once with respect to every
+    tensor; gradients repeat bit for bit.
+    """
+    if not residual.is_cuda or residual.dtype not in _TYPES or residual.dim() < 1:
+        raise ValueError("residual must be a float32, bfloat16 or float16 CUDA tensor")
+    shape, D, device = residual.shape, residual.shape[-1], residual.device
+    if not 0 < D <= 16384:
+        raise ValueError("rows must have 1 to 16384 features, got %d" % D)
+    if dtype is None:
+        dtype = residual.dtype if branch is None else branch.dtype
+    if post not in _NORMS or pre not in _NORMS:
+        raise ValueError('post and pre are "rms", "layer" or None')
+    if dtype not in _TYPES or residual.dtype not in (dtype, torch.float32):
+        raise ValueError("residual must be float32 or of the type of what the next block takes")
+    scale, factor = (residual_scale, 1.0) if isinstance(residual_scale, torch.Tensor) else (None, float(residual_scale))
+    gate_rows = rows = residual.numel() // D
+    if branch is None:
+        if gate is not None or scale is not None or factor != 1.0 or post is not None or pre is None:
+            raise ValueError("without a branch there is a norm before the next block and nothing else")
+    else:
+        if branch.shape != shape or branch.device != device or branch.dtype != dtype:
+            raise ValueError("branch must have residual's shape and device and the type of what the next block takes")
+        if gate is not None:
+            gate, gate_rows = _gate_rows(gate, shape)
+        if scale is not None and scale.shape != (D,):
+            scale = scale.reshape(-1).expand(D)
+    if (post is None and (post_weight is not None or post_bias is not None)) or \
+            (pre is None and (pre_weight is not None or pre_bias is not None)):
+        raise ValueError("a weight or a bias belongs to a norm")
+    params = (gate, scale, post_weight, post_bias, pre_weight, pre_bias)
+    tracked = residual.requires_grad or (branch is not None and branch.requires_grad)
+    for k, p in enumerate(params):
+        if p is not None:
+            if p.device != device or p.dtype not in _TYPES or (k > 0 and p.shape != (D,)):
+                raise ValueError("%s must be a float32, bfloat16 or float16 tensor [%d] on residual's device" % (_PARAMS[k], D))
+            tracked = tracked or p.requires_grad
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    conf = (factor, _NORMS[post], _NORMS[pre], eps, weight_offset, max(gate_rows, 1), dtype, pre is not None)
+    if torch.compiler.is_compiling() or type(residual) is not torch.Tensor and type(residual) is not torch.nn.Parameter:
+        total, out, _ = _block_norm_op(residual, branch, *params, *conf)
+        total, out = (None if branch is None else total), (None if pre is None else out)
+    elif tracked and torch.is_grad_enabled():
+        return _BlockNorm.apply(residual, branch, *params, conf)
+    else:
+        total, out, _ = _block_norm_forward(residual, branch, params, *conf, False)
+    return (residual if branch is None else total), out
+
+
+class NMBlockStack(torch.nn.Module):
+    """Blocks of a model around one residual stream, with a norm before and after each of them.
+
+    h = pre_0(x);  for every block i:  x = residual_scale * x + gate_i * post_i(block_i(h));  h = pre_{i+1}(x)
+    and returns (x, h), h normed for what follows the last block.  Block i's post norm, gate and sum and block i+1's pre
+    norm are one launch (block_norm).  blocks: modules [..., features] -> [..., features] (NMSparseLinear, NMQuantLinear or what is
+    built of them); norm: "rms" or "layer"; gate: give each block a learned gate per feature, which starts at gate_init;
+    dtype: the type of what the blocks take and return, x's own unless given (x may be float32 beside it).
+    """
+
+    def __init__(self, blocks, features, norm="rms", residual_scale=1.0, gate=False, gate_init=1.0, eps=1e-6, dtype=None, device="cuda"):
+        super().__init__()
+        if norm not in ("rms", "layer"):
+            raise ValueError('norm is "rms" or "layer"')
+        self.blocks = torch.nn.ModuleList(blocks)
+        self.norm, self.residual_scale, self.eps, self.dtype = norm, residual_scale, eps, dtype
+        count = len(self.blocks)
+
+        def vectors(n, value):
+            return torch.nn.ParameterList([torch.nn.Parameter(torch.full((features,), value, device=device)) for _ in range(n)])
+
+        self.pre_weight, self.post_weight = vectors(count + 1, 1.0), vectors(count, 1.0)
+        self.pre_bias = vectors(count + 1, 0.0) if norm == "layer" else None
+        self.post_bias = vectors(count, 0.0) if norm == "layer" else None
+        self.gate = vectors(count, gate_init) if gate else None
+
+    def _pre(self, i):
+        return dict(pre=self.norm, pre_weight=self.pre_weight[i], pre_bias=None if self.pre_bias is None else self.pre_bias[i], eps=self.eps)
+
+    def forward(self, x):
+        dtype = x.dtype if self.dtype is None else self.dtype
+        _, h = block_norm(x, dtype=dtype, **self._pre(0))
+        for i, block in enumerate(self.blocks):
+            x, h = block_norm(x, block(h), gate=None if self.gate is None else self.gate[i], residual_scale=self.residual_scale,
+                              post=self.norm, post_weight=self.post_weight[i],
+                              post_bias=None if self.post_bias is None else self.post_bias[i], dtype=dtype, **self._pre(i + 1))
+        return x, h
