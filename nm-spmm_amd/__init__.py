@@ -110,7 +110,9 @@ def lib():
         L.nmspmm_q4_quantize_device.argtypes = [c_void_p, c_void_p, op, ctypes.c_uint, c_void_p]
         L.nmspmm_q4_pack_device.argtypes = [c_void_p] * 4 + [op, c_void_p]
         L.nmspmm_q4_expand_device.argtypes = [op, c_void_p, c_void_p]
-        L.nmspmm_q4_linear.argtypes = [op, c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p]
+        L.nmspmm_q4_linear.argtypes = [op, c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p, c_size_t, c_void_p]
+        L.nmspmm_q4_workspace_bytes.restype = c_size_t
+        L.nmspmm_q4_workspace_bytes.argtypes = [c_int] * 6
         # (the two structs of the norms are packed bytes: BLOCK_NORM, BLOCK_NORM_GRADS)
         L.nmspmm_block_norm_forward.argtypes = [ctypes.c_char_p, c_void_p]
         L.nmspmm_block_norm_backward.argtypes = [ctypes.c_char_p, ctypes.c_char_p, c_void_p, c_size_t, c_void_p]
@@ -338,12 +340,18 @@ def q4_expand_device(op, dB):
     _check("nmspmm_q4_expand_device", lib().nmspmm_q4_expand_device(ctypes.byref(op), _ptr(dB), _stream()))
 
 
-def q4_linear(op, x, y, M, type, ldx=None, ldy=None):
+def q4_workspace_bytes(M, K, N, n=1, m=1, type=F32):
+    return lib().nmspmm_q4_workspace_bytes(M, K, N, n, m, type)
+
+
+def q4_linear(op, x, y, M, type, ldx=None, ldy=None, workspace=None):
     """y [M, N] = x [M, K] times the operand plus its bias; rows ldx and ldy elements apart."""
     ldx, ldy = op.K if ldx is None else ldx, op.N if ldy is None else ldy
     if M > 0:
         _need("q4_linear", x=(x, (M - 1) * ldx + op.K), y=(y, (M - 1) * ldy + op.N))
-    _check("nmspmm_q4_linear", lib().nmspmm_q4_linear(ctypes.byref(op), _ptr(x), ldx, _ptr(y), ldy, M, type, _stream()))
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _check("nmspmm_q4_linear",
+           lib().nmspmm_q4_linear(ctypes.byref(op), _ptr(x), ldx, _ptr(y), ldy, M, type, _ptr(workspace), ws_bytes, _stream()))
 
 
 # ---- host-pointer forms: arguments are C-contiguous numpy int32 arrays, updated in place ----------

@@ -17,7 +17,7 @@ int q4_shape(int K, int N, int n, int m, int group, Q4Shape* p)
         return NMSPMM_ERR_BAD_PATTERN;
     if (n != m && ((n != 1 && n != 2 && n != 4 && n != 8) || (m != 2 * n && m != 4 * n && m != 8 * n)))
         return NMSPMM_ERR_BAD_PATTERN;
-    if (K <= 0 || N <= 0 || K > (1 << 30) || N > (1 << 21))
+    if (K <= 0 || N <= 0 || K > (1 << 24) || N > (1 << 20))
         return NMSPMM_ERR_BAD_SHAPE;
     if (n != m && (K % m != 0 || N % 32 != 0))
         return NMSPMM_ERR_BAD_SHAPE;
@@ -76,6 +76,15 @@ size_t nmspmm_q4_row_offsets_bytes(int K, int N, int n, int m)
     return q4_shape(K, N, n, m, 128, &p) == NMSPMM_OK && p.m > 1 ? (size_t)(N / 32) * p.blocks * 128 : 0;
 }
 
+size_t nmspmm_q4_workspace_bytes(int M, int K, int N, int n, int m, int type)
+{
+    Q4Shape p;
+    if (M <= 0 || M > (1 << 24) || (type != NMSPMM_F32 && type != NMSPMM_BF16 && type != NMSPMM_F16) ||
+        q4_shape(K, N, n, m, 128, &p) != NMSPMM_OK)
+        return 0;
+    return q4_workspace_bytes(p, M, (ElementType)type);
+}
+
 int nmspmm_q4_quantize_device(const float* dBT, const int32_t* dDT, const nmspmm_q4_operand* op, unsigned flags, void* stream)
 {
     Q4Shape p;
@@ -124,7 +133,7 @@ int nmspmm_q4_expand_device(const nmspmm_q4_operand* op, float* dB, void* stream
 }
 
 int nmspmm_q4_linear(const nmspmm_q4_operand* op, const void* x, long long ldx, void* y, long long ldy, int M, int type,
-                     void* stream)
+                     void* workspace, size_t workspace_bytes, void* stream)
 {
     Q4Shape p;
     const int st = check_operand(op, &p);
@@ -132,7 +141,7 @@ int nmspmm_q4_linear(const nmspmm_q4_operand* op, const void* x, long long ldx, 
         return st;
     if (type != NMSPMM_F32 && type != NMSPMM_BF16 && type != NMSPMM_F16)
         return NMSPMM_ERR_BAD_PATTERN;
-    if (M < 0 || M > (1 << 30) || ldx < p.K || ldy < p.N)
+    if (M < 0 || M > (1 << 24) || ldx < p.K || ldy < p.N)
         return NMSPMM_ERR_BAD_SHAPE;
     if (M == 0)
         return NMSPMM_OK;
@@ -141,10 +150,21 @@ int nmspmm_q4_linear(const nmspmm_q4_operand* op, const void* x, long long ldx, 
     const size_t size = type == NMSPMM_F32 ? 4 : 2;
     if (!aligned(x, size) || !aligned(y, size))
         return NMSPMM_ERR_ALIGNMENT;
+    const size_t need = q4_workspace_bytes(p, M, (ElementType)type);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return NMSPMM_ERR_WORKSPACE;
+    if (need > 0 && !aligned(workspace, 16))
+        return NMSPMM_ERR_ALIGNMENT;
     Q4LinearArgs a;
     a.x = x;
     a.codes = (const uint32_t*)op->codes;
-    a.meta = (const uint32_t*)op->meta;
+    a.meta.words = (const uint32_t*)op->meta;
+    a.meta.blocks = p.blocks;
+    a.meta.per = 128 / p.group;
+    a.meta.per_shift = p.group == 128 ? 0 : p.group == 64 ? 1 : 2;
+    a.meta.group = p.group;
+    a.meta.group_shift = p.group == 128 ? 7 : p.group == 64 ? 6 : 5;
+    a.meta.last = (p.W - 1) / p.group;
     a.rows = offsets_of(op, p);
     a.bias = op->bias;
     a.y = y;
@@ -153,7 +173,7 @@ int nmspmm_q4_linear(const nmspmm_q4_operand* op, const void* x, long long ldx, 
     a.M = M;
     a.p = p;
     a.stream = (hipStream_t)stream;
-    return launch_q4_linear(a, (ElementType)type) == hipSuccess ? NMSPMM_OK : NMSPMM_ERR_HIP;
+    return launch_q4_linear(a, (ElementType)type, workspace) == hipSuccess ? NMSPMM_OK : NMSPMM_ERR_HIP;
 }
 
 } // extern "C"

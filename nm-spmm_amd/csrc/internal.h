@@ -566,10 +566,29 @@ struct Q4Shape {
 
 enum ElementType { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
+// Scales and zero points (layout: q4.hip), found by the rows that the operand is multiplied by: kept rows, or dense rows once
+// the codes of a sparse operand were filled up to those of a dense one (q4_gemm.hip).
+struct Q4Meta {
+    const uint32_t* words;
+    int blocks;         // of 128 kept rows
+    int per, per_shift; // words of a block and column, 1, 2 or 4, and its logarithm
+    int group;          // rows that share a word, 32 .. 1024
+    int group_shift;
+    int last;           // the last group
+#ifdef __HIPCC__
+    __device__ uint32_t word(int tile, int row, int c) const
+    {
+        const int j = min(row >> group_shift, last);    // rows beyond the operand's: x is zero there
+        // (what is the same for a wave stands apart from the column: a scalar address)
+        return (words + ((size_t)tile * blocks + (j >> per_shift)) * 16 * per + (j & (per - 1)))[c * per];
+    }
+#endif
+};
+
 struct Q4LinearArgs {
     const void* x;              // M rows of K elements, ldx elements apart
     const uint32_t* codes;
-    const uint32_t* meta;
+    Q4Meta meta;
     const uint8_t* rows;        // nullptr: dense
     const float* bias;          // N or nullptr
     void* y;                    // M rows of N elements of x's type, ldy elements apart
@@ -584,7 +603,13 @@ hipError_t launch_q4_pack(const float* values, const uint8_t* given, const float
                           uint8_t* row_offsets, hipStream_t stream);
 hipError_t launch_q4_expand(const uint32_t* codes, const uint32_t* meta, const uint8_t* row_offsets, const Q4Shape& p,
                             float* B, hipStream_t stream);
-hipError_t launch_q4_linear(const Q4LinearArgs& a, ElementType type);
+// The workspace holds what q4_workspace_bytes says; 0 bytes: it may be nullptr.
+size_t q4_workspace_bytes(const Q4Shape& p, int M, ElementType type);
+hipError_t launch_q4_linear(const Q4LinearArgs& a, ElementType type, void* workspace);
+bool q4_uses_gemm(const Q4Shape& p, int M);
+bool q4_densifies(const Q4Shape& p, int M);
+hipError_t launch_q4_densify(const Q4LinearArgs& a, uint32_t* out);
+hipError_t launch_q4_gemm(const Q4LinearArgs& a, ElementType type, bool densified, void* workspace);
 
 // ---- the norms around a block (block_norm.hip) ---------------------------------------------------------
 

@@ -195,8 +195,17 @@ q4_rows_kernel(const int32_t* __restrict__ rows, Q4Shape p, uint8_t* __restrict_
     int offset = 0;
     if (r < p.W) {
         int local = rows[i];
-        if (local < 0 || local >= p.m)
-            local = 0;                  // its code is the zero point
+        if (local < 0 || local >= p.m) {
+            // its code is the zero point: any row that the window does not keep will do
+            const int first = r / p.n * p.n;
+            for (local = 0; local < p.m; ++local) {
+                bool kept = false;
+                for (int k = 0; k < p.n; ++k)
+                    kept |= rows[(size_t)(first + k) * Q + v] == local;
+                if (!kept)
+                    break;
+            }
+        }
         offset = dense_row(r, p.n, p.m, local) - (r >> 5) * p.span;
     }
     out[(size_t)v * p.blocks * 128 + r] = (uint8_t)offset;

@@ -1,0 +1,46 @@
+// Device code that the products with 4-bit operands share (q4_linear.hip, q4_gemm.hip).
+#ifndef NMSPMM_Q4_DEVICE_H
+#define NMSPMM_Q4_DEVICE_H
+
+#include "internal.h"
+
+namespace nmspmm {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <ElementType T>
+__device__ inline f32x4 product(u32x4 a, u32x4 b, f32x4 c)
+{
+    if (T == kF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Eight codes -> eight operand elements 16 + code.
+template <ElementType T>
+__device__ inline u32x4 widened(uint32_t w)
+{
+    if (T == kF16) {
+        const uint32_t mask = 0x03c003c0u, one = 0x4c004c00u;
+        return u32x4{((w << 6) & mask) | one, ((w << 2) & mask) | one, ((w >> 2) & mask) | one, ((w >> 6) & mask) | one};
+    }
+    const uint32_t mask = 0x00780078u, one = 0x41804180u;
+    return u32x4{((w << 3) & mask) | one, ((w >> 1) & mask) | one, ((w >> 5) & mask) | one, ((w >> 9) & mask) | one};
+}
+
+template <ElementType T>
+__device__ inline void store_result(void* y, size_t at, float v)
+{
+    if (T == kF32)
+        static_cast<float*>(y)[at] = v;
+    else if (T == kBF16)
+        static_cast<uint16_t*>(y)[at] = __builtin_bit_cast(uint16_t, (__bf16)v);
+    else
+        static_cast<uint16_t*>(y)[at] = __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+
+} // namespace nmspmm
+#endif

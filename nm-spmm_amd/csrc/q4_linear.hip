@@ -10,55 +10,15 @@
 // tile for row i of x) and are added at the end, so no activation is rounded.
 // An infinity or a NaN in a row of x makes that row of y NaN.
 #include "internal.h"
+#include "q4_device.h"
 
 namespace nmspmm {
 
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
 constexpr int kMaxWaves = 16;
 constexpr int kRowPitch = 136;      // 16-bit elements between staged rows: 128 and 16 bytes, so that the sixteen
                                     // rows of a 128-bit LDS read start in different banks
-
-template <ElementType T>
-__device__ inline f32x4 product(u32x4 a, u32x4 b, f32x4 c)
-{
-    if (T == kF16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// Eight codes -> eight operand elements 16 + code.
-template <ElementType T>
-__device__ inline u32x4 widened(uint32_t w)
-{
-    if (T == kF16) {
-        const uint32_t mask = 0x03c003c0u, one = 0x4c004c00u;
-        return u32x4{((w << 6) & mask) | one, ((w << 2) & mask) | one, ((w >> 2) & mask) | one, ((w >> 6) & mask) | one};
-    }
-    const uint32_t mask = 0x00780078u, one = 0x41804180u;
-    return u32x4{((w << 3) & mask) | one, ((w >> 1) & mask) | one, ((w >> 5) & mask) | one, ((w >> 9) & mask) | one};
-}
-
-__device__ inline uint16_t to_bits(float v, ElementType t)
-{
-    if (t == kBF16)
-        return __builtin_bit_cast(uint16_t, (__bf16)v);
-    return __builtin_bit_cast(uint16_t, (_Float16)v);
-}
-
-template <ElementType T>
-__device__ inline void store_result(void* y, size_t at, float v)
-{
-    if (T == kF32)
-        static_cast<float*>(y)[at] = v;
-    else
-        static_cast<uint16_t*>(y)[at] = to_bits(v, T);
-}
 
 // How the activations reach the matrix operands: as they lie in memory (16-bit types, 16-byte aligned rows of whole
 // 8-element pieces), or through the wave's own part of LDS, from consecutive or from gathered elements.
@@ -69,7 +29,7 @@ enum Source { kDirect, kStaged, kGathered };
 template <ElementType T, Source SRC, int RT, int NC, int MX>
 __global__ void __launch_bounds__(kMaxWaves * 64)
 q4_rows_product_kernel(const void* __restrict__ x_, size_t ldx, const uint32_t* __restrict__ codes,
-                       const uint32_t* __restrict__ meta, const uint8_t* __restrict__ rows, const float* __restrict__ bias,
+                       Q4Meta meta, const uint8_t* __restrict__ rows, const float* __restrict__ bias,
                        void* __restrict__ y, size_t ldy, int M, Q4Shape p, bool pairs)
 {
     constexpr int S = T == kF32 ? 3 : 1;              // staged rows per row of x
@@ -81,7 +41,8 @@ q4_rows_product_kernel(const void* __restrict__ x_, size_t ldx, const uint32_t* 
     const int c = lane & 15, kb = lane >> 4;
     const int tile0 = blockIdx.x * NC, m0 = blockIdx.y * Chunk;
     const int rows_here = min(Chunk, M - m0);
-    const int per = 128 / p.group, step_mask = p.group / 32 - 1, per_shift = per == 4 ? 0 : per == 2 ? 1 : 2;
+    // groups of 128 rows and more are scaled once a block, smaller ones when they end
+    const int units = meta.group < 128 ? 128 / meta.group : 1, step_mask = 4 / units - 1, unit_shift = units == 4 ? 0 : units == 2 ? 1 : 2;
     uint16_t* const stage = reinterpret_cast<uint16_t*>(lds) + (size_t)wave * (MX * S * kRowPitch);
 
     f32x4 total[RT][NC], acc[RT][NC], ones[RT];
@@ -95,21 +56,17 @@ q4_rows_product_kernel(const void* __restrict__ x_, size_t ldx, const uint32_t* 
     const uint32_t unit = T == kF16 ? 0x3c003c00u : 0x3f803f80u;
     const u32x4 unit8 = u32x4{unit, unit, unit, unit};
 
-    u32x4 w[NC], mt[NC], xd[RT][4];
+    u32x4 w[NC], mt[NC] = {}, xd[RT][4];
     uint32_t xs[MX][2];
     auto load = [&](int b) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             const size_t at = (size_t)(tile0 + j) * p.blocks + b;
             w[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(codes) + at * 64 + lane);
-            const uint32_t* const ms = meta + (at * 16 + c) * per;
-            if (per == 4)
-                mt[j] = *reinterpret_cast<const u32x4*>(ms);
-            else if (per == 2) {
-                const uint2 two = *reinterpret_cast<const uint2*>(ms);
-                mt[j] = u32x4{two.x, two.y, 0, 0};
-            } else
-                mt[j] = u32x4{ms[0], 0, 0, 0};
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (g < units)
+                    mt[j][g] = meta.word(tile0 + j, b * 128 + g * meta.group, c);
         }
         if (SRC == kDirect) {
             const uint16_t* const x = static_cast<const uint16_t*>(x_);
@@ -224,7 +181,7 @@ q4_rows_product_kernel(const void* __restrict__ x_, size_t ldx, const uint32_t* 
                     acc[t][j] = product<T>(xa[t][s], u, acc[t][j]);
             }
             if ((s & step_mask) == step_mask) {     // the group ends with this step
-                const int g = s >> per_shift;
+                const int g = s >> unit_shift;
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
                     const uint32_t word = g == 0 ? mn[j][0] : g == 1 ? mn[j][1] : g == 2 ? mn[j][2] : mn[j][3];
@@ -297,6 +254,11 @@ hipError_t launch_rows(const Q4LinearArgs& a, bool pairs)
 template <ElementType T, Source SRC>
 hipError_t launch_source(const Q4LinearArgs& a, bool pairs)
 {
+    if (SRC == kDirect) {
+        if (a.M <= 16)
+            return launch_rows<T, SRC, 1, 1, 1>(a, pairs);
+        return a.M <= 32 ? launch_rows<T, SRC, 2, 1, 1>(a, pairs) : launch_rows<T, SRC, 4, 1, 1>(a, pairs);
+    }
     if (a.M == 1)
         return launch_rows<T, SRC, 1, 1, 1>(a, pairs);
     return launch_rows<T, SRC, 1, 1, T == kF32 ? 4 : 16>(a, pairs);
@@ -304,8 +266,24 @@ hipError_t launch_source(const Q4LinearArgs& a, bool pairs)
 
 } // namespace
 
-hipError_t launch_q4_linear(const Q4LinearArgs& a, ElementType type)
+hipError_t launch_q4_linear(const Q4LinearArgs& given, ElementType type, void* workspace)
 {
+    Q4LinearArgs a = given;
+    const bool densified = q4_densifies(a.p, a.M);
+    if (densified) {
+        const hipError_t e = launch_q4_densify(a, static_cast<uint32_t*>(workspace));
+        if (e != hipSuccess)
+            return e;
+        a.codes = static_cast<const uint32_t*>(workspace);
+        a.meta.group = a.meta.group * a.p.m / a.p.n;
+        while ((1 << a.meta.group_shift) < a.meta.group)
+            ++a.meta.group_shift;
+        a.rows = nullptr;
+        a.p.W = a.p.K;
+        a.p.blocks = (a.p.K + 127) / 128;
+    }
+    if (q4_uses_gemm(a.p, a.M))
+        return launch_q4_gemm(a, type, densified, workspace);
     const size_t size = type == kF32 ? 4 : 2;
     const uintptr_t base = reinterpret_cast<uintptr_t>(a.x);
     // a lane's two neighbouring elements in one load
@@ -318,7 +296,7 @@ hipError_t launch_q4_linear(const Q4LinearArgs& a, ElementType type)
     if (type == kF32)
         return launch_source<kF32, kStaged>(a, pairs);
     if (base % 16 == 0 && a.ldx % 8 == 0 && a.p.K % 8 == 0)
-        return type == kBF16 ? launch_rows<kBF16, kDirect, 1, 1, 1>(a, pairs) : launch_rows<kF16, kDirect, 1, 1, 1>(a, pairs);
+        return type == kBF16 ? launch_source<kBF16, kDirect>(a, pairs) : launch_source<kF16, kDirect>(a, pairs);
     return type == kBF16 ? launch_source<kBF16, kStaged>(a, pairs) : launch_source<kF16, kStaged>(a, pairs);
 }
 

@@ -235,7 +235,13 @@ def _quant_linear(x, operand):
 
 
 def _launch_quant_linear(x, ldx, y, ldy, M, operand, device):
-    status = _nm.lib().nmspmm_q4_linear(operand, x.data_ptr(), ldx, y.data_ptr(), ldy, M, _TYPES[x.dtype], _on(device))
+    type_, need, space = _TYPES[x.dtype], 0, None
+    if M > 16:      # below, no operand needs a workspace
+        need = _nm.lib().nmspmm_q4_workspace_bytes(M, operand.K, operand.N, operand.n, operand.m, type_)
+        if need:
+            workspace = x.new_empty(need, dtype=torch.uint8)    # from torch's caching allocator, ordered on the stream
+            space = workspace.data_ptr()
+    status = _nm.lib().nmspmm_q4_linear(operand, x.data_ptr(), ldx, y.data_ptr(), ldy, M, type_, space, need, _on(device))
     if status != _nm.OK:
         raise _nm.NmSpmmError("nmspmm_q4_linear", status)
     return y

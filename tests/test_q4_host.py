@@ -22,7 +22,7 @@ def test_buffer_sizes():
     assert nmspmm.q4_row_offsets_bytes(4096, 4096, 2, 8) == 1024 * 128
     assert nmspmm.q4_row_offsets_bytes(4096, 4096) == 0
     for bad in ((0, 64, 1, 1), (256, 0, 1, 1), (256, 64, 3, 8), (256, 64, 2, 32), (256, 64, 16, 32), (250, 64, 2, 4), (256, 48, 2, 4),
-                (256, 64, 4, 2), (256, 64, 0, 4), (256, 64, -2, -4), ((1 << 30) + 1, 64, 1, 1), (64, (1 << 21) + 1, 1, 1)):
+                (256, 64, 4, 2), (256, 64, 0, 4), (256, 64, -2, -4), ((1 << 24) + 1, 64, 1, 1), (64, (1 << 20) + 1, 1, 1)):
         assert nmspmm.q4_codes_bytes(*bad) == 0 and nmspmm.q4_meta_bytes(*bad) == 0 and nmspmm.q4_row_offsets_bytes(*bad) == 0
     for group in (0, 16, 48, 256, -32):
         assert nmspmm.q4_meta_bytes(256, 64, 1, 1, group) == 0
@@ -34,7 +34,7 @@ def test_buffer_sizes():
     (dict(codes=0x10004), 8), (dict(meta=0x10008), 8), (dict(n=2, m=4, rows=0x10001), 8), (dict(bias=0x10002), 8)])
 def test_every_entry_point_refuses_a_bad_operand(op, status):
     L, o = nmspmm.lib(), operand(**op)
-    assert L.nmspmm_q4_linear(o, FAKE, 1 << 20, FAKE, 1 << 20, 1, 0, None) == status
+    assert L.nmspmm_q4_linear(o, FAKE, 1 << 20, FAKE, 1 << 20, 1, 0, None, 0, None) == status
     assert L.nmspmm_q4_quantize_device(FAKE, FAKE, o, 0, None) == status
     assert L.nmspmm_q4_pack_device(FAKE, FAKE, None, FAKE, o, None) == status
     assert L.nmspmm_q4_expand_device(o, FAKE, None) == status
@@ -42,16 +42,24 @@ def test_every_entry_point_refuses_a_bad_operand(op, status):
 
 def test_refusals_of_the_other_arguments():
     L, dense, sparse = nmspmm.lib(), operand(), operand(n=2, m=4)
-    assert L.nmspmm_q4_linear(None, FAKE, 256, FAKE, 64, 1, 0, None) == 1
-    assert L.nmspmm_q4_linear(dense, None, 256, FAKE, 64, 1, 0, None) == 1
-    assert L.nmspmm_q4_linear(dense, FAKE, 256, None, 64, 1, 0, None) == 1
-    assert L.nmspmm_q4_linear(dense, None, 256, None, 64, 0, 0, None) == 0      # no rows: nothing to do
-    assert L.nmspmm_q4_linear(dense, FAKE, 255, FAKE, 64, 1, 0, None) == 2
-    assert L.nmspmm_q4_linear(dense, FAKE, 256, FAKE, 63, 1, 0, None) == 2
-    assert L.nmspmm_q4_linear(dense, FAKE, 256, FAKE, 64, -1, 0, None) == 2
-    assert L.nmspmm_q4_linear(dense, FAKE, 256, FAKE, 64, 1, 3, None) == 3
-    assert L.nmspmm_q4_linear(dense, ctypes.c_void_p(0x10002), 256, FAKE, 64, 1, 0, None) == 8
-    assert L.nmspmm_q4_linear(dense, ctypes.c_void_p(0x10001), 256, FAKE, 64, 1, 1, None) == 8
+    assert L.nmspmm_q4_linear(None, FAKE, 256, FAKE, 64, 1, 0, None, 0, None) == 1
+    assert L.nmspmm_q4_linear(dense, None, 256, FAKE, 64, 1, 0, None, 0, None) == 1
+    assert L.nmspmm_q4_linear(dense, FAKE, 256, None, 64, 1, 0, None, 0, None) == 1
+    assert L.nmspmm_q4_linear(dense, None, 256, None, 64, 0, 0, None, 0, None) == 0      # no rows: nothing to do
+    assert L.nmspmm_q4_linear(dense, FAKE, 255, FAKE, 64, 1, 0, None, 0, None) == 2
+    assert L.nmspmm_q4_linear(dense, FAKE, 256, FAKE, 63, 1, 0, None, 0, None) == 2
+    assert L.nmspmm_q4_linear(dense, FAKE, 256, FAKE, 64, -1, 0, None, 0, None) == 2
+    assert L.nmspmm_q4_linear(dense, FAKE, 256, FAKE, 64, 1, 3, None, 0, None) == 3
+    assert L.nmspmm_q4_linear(dense, ctypes.c_void_p(0x10002), 256, FAKE, 64, 1, 0, None, 0, None) == 8
+    assert L.nmspmm_q4_linear(dense, ctypes.c_void_p(0x10001), 256, FAKE, 64, 1, 1, None, 0, None) == 8
+    many = nmspmm.q4_workspace_bytes(65, 256, 64, 1, 1, 0)
+    assert many > 0 and nmspmm.q4_workspace_bytes(64, 256, 64, 1, 1, 0) == 0
+    assert nmspmm.q4_workspace_bytes(17, 256, 64, 2, 4, 1) == 256 * 64 // 2 and nmspmm.q4_workspace_bytes(16, 256, 64, 2, 4, 1) == 0
+    for bad in ((0, 256, 64, 1, 1, 0), (-1, 256, 64, 1, 1, 0), (65, 256, 64, 1, 1, 3), (65, 0, 64, 1, 1, 0), (65, 256, 64, 3, 8, 0)):
+        assert nmspmm.q4_workspace_bytes(*bad) == 0
+    assert L.nmspmm_q4_linear(dense, FAKE, 256, FAKE, 64, 65, 0, None, 0, None) == 6
+    assert L.nmspmm_q4_linear(dense, FAKE, 256, FAKE, 64, 65, 0, FAKE, many - 1, None) == 6
+    assert L.nmspmm_q4_linear(dense, FAKE, 256, FAKE, 64, 65, 0, ctypes.c_void_p(0x10008), many, None) == 8
     assert L.nmspmm_q4_quantize_device(None, None, dense, 0, None) == 1
     assert L.nmspmm_q4_quantize_device(FAKE, None, sparse, 0, None) == 1
     assert L.nmspmm_q4_quantize_device(FAKE, None, dense, 2, None) == 2
