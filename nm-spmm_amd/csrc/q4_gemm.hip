@@ -247,23 +247,28 @@ q4_gemm_kernel(GemmArgs g)
                 fetch_codes(b);
             }
         }
+        // the sums of a unit are scaled when it ends; the pieces of one fp32 x share the sum of x, which is taken off once
+        const bool last = qq == PLANES - 1;
+#pragma clang loop unroll(disable)
+        for (int u = 0; u < UNITS; ++u) {       // (unrolled, smaller units would need more registers than there are)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            u32x4 a[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                a[t] = *reinterpret_cast<const u32x4*>(tile[half] + (t * 16 + c) * 256 + (((s * 4 + kb) ^ c) * 16));
-#pragma unroll
-            for (int j = 0; j < NC; ++j) {
-                const u32x4 u = widened<T>(w[j][s]);
+            for (int i = 0; i < Steps; ++i) {
+                const int s = u * Steps + i;
+                u32x4 a[4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
-                    acc[t][j] = product<T>(a[t], u, acc[t][j]);
+                    a[t] = *reinterpret_cast<const u32x4*>(tile[half] + (t * 16 + c) * 256 + (((s * 4 + kb) ^ c) * 16));
+#pragma unroll
+                for (int j = 0; j < NC; ++j) {
+                    const uint32_t word = UNITS == 1 ? w[j][i] : UNITS == 2 ? (u ? w[j][i + 2] : w[j][i])
+                                                     : u == 0 ? w[j][0] : u == 1 ? w[j][1] : u == 2 ? w[j][2] : w[j][3];
+                    const u32x4 wide = widened<T>(word);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        acc[t][j] = product<T>(a[t], wide, acc[t][j]);
+                }
             }
-            // the sums of a unit are scaled when it ends; the pieces of one fp32 x share the sum of x, which is taken off once
-            const bool last = qq == PLANES - 1;
-            if (s % Steps == Steps - 1 && (last || UNITS > 1)) {
-                const int u = s / Steps;
+            if (last || UNITS > 1) {
                 f32x4 xs[4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
@@ -273,7 +278,8 @@ q4_gemm_kernel(GemmArgs g)
                 }
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
-                    const uint32_t word = mt[j][u];
+                    const uint32_t word = UNITS == 1 ? mt[j][0] : UNITS == 2 ? (u ? mt[j][UNITS - 1] : mt[j][0])
+                                                     : u == 0 ? mt[j][0] : u == 1 ? mt[j][1 % UNITS] : u == 2 ? mt[j][2 % UNITS] : mt[j][3 % UNITS];
                     const float scale = __uint_as_float(word & ~15u);
                     const float offset = -(16.0f + (float)(word & 15u));
 #pragma unroll
