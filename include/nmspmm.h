@@ -332,7 +332,7 @@ int nmspmm_gemm_auto(const float* A, const float* B, const int32_t* D, const int
  * is what bounds it: 4 bits, and 4 bytes a group, in place of 32 bits.
  * Patterns: n == m (dense: any K and N), or n in {1, 2, 4, 8} kept rows in every window of m = 2 n, 4 n
  * or 8 n (K % m == 0, N % 32 == 0, one index pattern per 32 columns, as everywhere in this library);
- * group 32, 64 or 128; K and M up to 2^24, N up to 2^20.
+ * group 32, 64 or 128; K up to 2^22, N up to 2^20, M up to 2^24.
  * The buffers are made once, by nmspmm_q4_quantize_device or nmspmm_q4_pack_device, in the layout that
  * the kernels read; they belong to the caller, who gives them the sizes that the three functions below
  * return and 16-byte alignment.  `bias` (float[N] or NULL) is added by nmspmm_q4_linear.  The struct is
@@ -373,8 +373,8 @@ int nmspmm_q4_expand_device(const nmspmm_q4_operand* op, float* dB, void* stream
  * `type`; sums in fp32, one rounding at the end.  M == 0 does nothing.  fp32 activations are multiplied
  * exactly (three bf16 pieces each), so the result is as near as an fp32 product's.  A row of x that
  * holds an infinity or a NaN, or magnitudes beyond 2^100, gives a row of NaN.  x and y must not overlap.
- * The workspace (16-byte aligned) holds what nmspmm_q4_workspace_bytes says, which is 0 for up to 64 rows times a dense and
- * 16 rows times a sparse operand (it may be NULL then).  Calls that may overlap in time take workspaces of their own;
+ * The workspace (16-byte aligned) holds what nmspmm_q4_workspace_bytes says, which is 0 for up to 4 rows (it may be NULL
+ * then).  Calls that may overlap in time take workspaces of their own;
  * nothing is kept in one from call to call.  No library state: any streams and threads; may be captured into a HIP graph.
  * Results repeat bit for bit. */
 typedef enum nmspmm_type { NMSPMM_F32 = 0, NMSPMM_BF16 = 1, NMSPMM_F16 = 2 } nmspmm_type;

@@ -17,7 +17,7 @@ int q4_shape(int K, int N, int n, int m, int group, Q4Shape* p)
         return NMSPMM_ERR_BAD_PATTERN;
     if (n != m && ((n != 1 && n != 2 && n != 4 && n != 8) || (m != 2 * n && m != 4 * n && m != 8 * n)))
         return NMSPMM_ERR_BAD_PATTERN;
-    if (K <= 0 || N <= 0 || K > (1 << 24) || N > (1 << 20))
+    if (K <= 0 || N <= 0 || K > (1 << 22) || N > (1 << 20))
         return NMSPMM_ERR_BAD_SHAPE;
     if (n != m && (K % m != 0 || N % 32 != 0))
         return NMSPMM_ERR_BAD_SHAPE;

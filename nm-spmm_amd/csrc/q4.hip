@@ -14,7 +14,7 @@
 //         the low four.
 //   rows  [N / 32][blocks * 128] uint8 (n < m only): the dense row of each kept row, counted from the
 //         first row of the windows of its k-step (32 kept rows span 32 m / n <= 256 dense rows).
-// Rows beyond W and columns beyond N are filled in (code 8, meta 0, offset 0).
+// Rows beyond W and columns beyond N are filled in (the group's zero point, meta 0, offset 0).
 #include "internal.h"
 
 namespace nmspmm {
@@ -118,7 +118,7 @@ q4_pack_kernel(const float* __restrict__ values, const uint8_t* __restrict__ giv
                     const float over = fmaf(-(f + 0.5f), scale, v[s][e]);
                     q = over > 0.0f ? f + 1.0f : over < 0.0f ? f : 2.0f * rintf(0.5f * f + 0.25f);
                 }
-                q = fminf(fmaxf(q + zero, 0.0f), 15.0f);
+                q = row0 + s * 32 + e < p.W ? fminf(fmaxf(q + zero, 0.0f), 15.0f) : zero;
                 w |= (uint32_t)q << (4 * ((e >> 1) + 4 * (e & 1)));
             }
             word[s] = w;
@@ -145,7 +145,7 @@ q4_pack_kernel(const float* __restrict__ values, const uint8_t* __restrict__ giv
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int r = row0 + s * 32 + e;
-                uint32_t q = 8u;
+                uint32_t q = z;      // rows beyond W count as zero
                 if (column && r < p.W) {
                     q = given[(size_t)r * p.N + col] & 15u;
                     if (rows) {     // a kept row outside its window counts as zero

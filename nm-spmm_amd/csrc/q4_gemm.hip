@@ -13,12 +13,9 @@ namespace nmspmm {
 
 namespace {
 
-constexpr int kRows = 64;               // rows of x per workgroup
-constexpr int kTileBytes = kRows * 256; // a 64 x 128 tile of x
-
 // ---- x: its pieces, and its sums over the dense rows of each group (at most 128 at a time) ---------------
 
-// One wave per 512 elements of a row, eight each lane.  PLANES 0: only the sums.  Pieces: [plane][row][K filled up to 128].
+// One wave per 512 elements of a row, eight each lane.  PLANES 0: only the sums.  Pieces: [row][plane][K filled up to 128].
 template <ElementType T, int PLANES>
 __global__ void __launch_bounds__(256)
 q4_prepare_x_kernel(const void* __restrict__ x_, size_t ldx, int M, int K, int Kp, int unit, uint16_t* __restrict__ planes,
@@ -74,7 +71,7 @@ q4_prepare_x_kernel(const void* __restrict__ x_, size_t ldx, int M, int K, int K
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 w[e] = __builtin_amdgcn_perm(v[2 * e + 1], v[2 * e], 0x07060302u);
-            *reinterpret_cast<u32x4*>(planes + ((size_t)q * M + row) * Kp + k0) = w;
+            *reinterpret_cast<u32x4*>(planes + ((size_t)row * 3 + q) * Kp + k0) = w;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 v[e] = __float_as_uint(__uint_as_float(v[e]) - __uint_as_float(v[e] & 0xffff0000u));
@@ -126,7 +123,7 @@ q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict
 // ---- the product --------------------------------------------------------------------------------------------
 
 struct GemmArgs {
-    const uint16_t* x;      // [plane][M][ldx]
+    const uint16_t* x;      // rows ldx elements apart, their planes `plane`; 64 rows within 2 GiB
     size_t plane, ldx;
     const float* sums;      // [K / unit][sums_ld]
     size_t sums_ld;
@@ -135,18 +132,29 @@ struct GemmArgs {
     const float* bias;
     void* y;
     size_t ldy;
+    float* partial;         // [split][M][partial_ld] where K is split
+    size_t partial_ld;
     int M, N, Kx;           // Kx: elements of a row of x, a multiple of 128
     int blocks, unit;       // dense blocks of 128 rows; rows after which sums are scaled (32, 64, 128)
+    int splits;
     int tiles, tiles_m, tiles_n;    // 16-column tiles of the operand; workgroups along rows and columns
 };
 
-// UNITS: how often in a block of 128 rows sums are scaled, 128 / unit.
-template <ElementType T, int PLANES, ElementType OUT, int NC, int UNITS>
+// A workgroup computes 16 RT rows x 64 NC columns of a range of K.  A stage is 128 dense rows, or 64 with the three pieces of an fp32 x
+// beside each other: a code is widened once for all of them.  STEPS: 32-row steps of a unit.
+template <ElementType T, int PLANES, ElementType OUT, int RT, int NC, int STEPS>
 __global__ void __launch_bounds__(256, 2)
 q4_gemm_kernel(GemmArgs g)
 {
-    __shared__ __attribute__((aligned(16))) unsigned char tile[2][kTileBytes];
-    __shared__ __attribute__((aligned(16))) float sums[2][UNITS][kRows];
+    constexpr int Rows = 16 * RT;
+    constexpr int StageSteps = PLANES == 1 ? 4 : 2;                         // 32-row steps of a stage
+    constexpr int Loops = StageSteps > STEPS ? StageSteps / STEPS : 1;      // units (or the part of one) in a stage
+    constexpr int LoopSteps = StageSteps / Loops;
+    constexpr int Pieces = PLANES * StageSteps * 4;                         // 16-byte pieces of a row in a stage
+    constexpr int RowBytes = Pieces * 16;
+    constexpr int Mine = (Rows * Pieces + 255) / 256;                       // pieces that a thread brings
+    __shared__ __attribute__((aligned(16))) unsigned char tile[2][Rows * RowBytes];
+    __shared__ __attribute__((aligned(16))) float sums[2][Loops][Rows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, kb = lane >> 4;
 
@@ -158,132 +166,153 @@ q4_gemm_kernel(GemmArgs g)
     const int id = die * share + min(die, extra) + place;
     const int band = id / (8 * g.tiles_n), inside = id - band * 8 * g.tiles_n;
     const int height = min(8, g.tiles_m - band * 8);
-    const int m0 = (band * 8 + inside % height) * kRows, tile0 = (inside / height) * (4 * NC) + wave * NC;
-    const int rows_here = min(kRows, g.M - m0);
+    const int m0 = (band * 8 + inside % height) * Rows, tile0 = (inside / height) * (4 * NC) + wave * NC;
+    const int rows_here = min(Rows, g.M - m0);
+    const int first_block = (int)((long long)g.blocks * blockIdx.y / g.splits);
+    const int end_block = (int)((long long)g.blocks * (blockIdx.y + 1) / g.splits);
+    const int first = first_block * 4 / StageSteps, end = end_block * 4 / StageSteps;   // stages
 
-    f32x4 acc[4][NC], total[4][NC];
+    f32x4 acc[RT][NC], total[RT][NC];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int j = 0; j < NC; ++j)
             acc[t][j] = total[t][j] = f32x4{0, 0, 0, 0};
 
-    // this lane's 16-byte pieces of a tile of x: rows 16 wave + 4 i + lane / 16, the piece that belongs at place lane % 16
-    uint32_t piece[4];
+    // Where piece q of row r lies in a row of the tile: swapped so that the sixteen rows of a read start in different banks.
+    auto place_of = [&](int r, int q) {
+        return PLANES == 1 ? q ^ (r & 15) : (q & ~7) | ((q ^ (r >> 1)) & 7);
+    };
+    uint32_t from[Mine], to[Mine];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = wave * 16 + i * 4 + kb;
-        piece[i] = (uint32_t)(row * g.ldx * 2) + ((c ^ (row & 15)) * 16);
+    for (int i = 0; i < Mine; ++i) {
+        const int n = i * 256 + threadIdx.x;
+        const int r = n / Pieces, q = n % Pieces;
+        // (a piece more than there are, or of a row beyond M: read as zero, and the former is not put down)
+        from[i] = (uint32_t)((q / (StageSteps * 4)) * g.plane * 2 + r * g.ldx * 2 + (q % (StageSteps * 4)) * 16);
+        if (r >= rows_here)
+            from[i] = 0x80000000u;
+        to[i] = (uint32_t)(r * RowBytes + place_of(r, q) * 16);
     }
     // Through registers and not straight into LDS: behind such a load the compiler lets every LDS read wait for it.
-    u32x4 xr[4];
+    u32x4 xr[Mine];
     uint32_t sr = 0;
-    auto fetch_x = [&](int b, int q) {
-        const uint16_t* const base = g.x + q * g.plane + (size_t)m0 * g.ldx + b * 128;
-        const uint32_t bytes = (uint32_t)(((size_t)(rows_here - 1) * g.ldx + (g.Kx - b * 128)) * 2);    // rows beyond M read as zero
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)bytes, 0x00020000);
+    auto fetch_x = [&](int stage) {
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(g.x + (size_t)m0 * g.ldx + stage * (StageSteps * 32)), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            xr[i] = __builtin_amdgcn_raw_buffer_load_b128(r, (int)piece[i], 0, 0);
+        for (int i = 0; i < Mine; ++i)
+            xr[i] = __builtin_amdgcn_raw_buffer_load_b128(r, (int)from[i], 0, 0);
     };
     auto put_x = [&](int half) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<u32x4*>(tile[half] + (wave * 16 + i * 4) * 256 + lane * 16) = xr[i];
+        for (int i = 0; i < Mine; ++i)
+            if (Rows * Pieces % 256 == 0 || i * 256 + (int)threadIdx.x < Rows * Pieces)
+                *reinterpret_cast<u32x4*>(tile[half] + to[i]) = xr[i];
     };
-    auto fetch_sums = [&](int b) {
-        if (wave < UNITS) {
-            const float* const base = g.sums + (size_t)(b * UNITS + wave) * g.sums_ld + m0;
+    auto fetch_sums = [&](int stage) {
+        if (wave < Loops) {
+            const int unit = (stage * StageSteps + wave * LoopSteps) / STEPS;
+            const float* const base = g.sums + (size_t)unit * g.sums_ld + m0;
             const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, rows_here * 4, 0x00020000);
             sr = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, 0, 0);
         }
     };
-    auto put_sums = [&](int b) {
-        if (wave < UNITS)
-            sums[b & 1][wave][lane] = __uint_as_float(sr);
+    auto put_sums = [&](int half) {
+        if (wave < Loops && lane < Rows)
+            sums[half][wave][lane] = __uint_as_float(sr);
     };
-    constexpr int Steps = 4 / UNITS;    // of 32 rows in a unit
-    u32x4 w[NC], wn[NC];
-    uint32_t mt[NC][UNITS];
-    auto fetch_codes = [&](int b) {
+    uint32_t w[NC][StageSteps], wn[NC][StageSteps], mt[NC][Loops];
+    auto fetch_codes = [&](int stage) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             const int t = min(tile0 + j, g.tiles - 1);      // beyond the last column: read, not used
-            wn[j] = (reinterpret_cast<const u32x4*>(g.codes) + ((size_t)t * g.blocks + b) * 64)[lane];
+            const int b = stage * StageSteps / 4;
+            const uint32_t* const base = g.codes + ((size_t)t * g.blocks + b) * 256 + (PLANES == 1 ? 0 : (stage & 1) * 2) + lane * 4;
+            if (PLANES == 1) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(base);
+#pragma unroll
+                for (int s = 0; s < StageSteps; ++s)
+                    wn[j][s] = v[s];
+            } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(base);
+                wn[j][0] = v.x;
+                wn[j][1] = v.y;
+            }
         }
     };
-    auto fetch_meta = [&](int b) {
+    auto fetch_meta = [&](int stage) {
 #pragma unroll
         for (int j = 0; j < NC; ++j)
 #pragma unroll
-            for (int u = 0; u < UNITS; ++u)
-                mt[j][u] = g.meta.word(min(tile0 + j, g.tiles - 1), b * 128 + u * (128 / UNITS), c);
+            for (int u = 0; u < Loops; ++u)
+                mt[j][u] = g.meta.word(min(tile0 + j, g.tiles - 1), (stage * StageSteps + u * LoopSteps) * 32, c);
     };
 
-    fetch_x(0, 0);
-    fetch_sums(0);
-    fetch_codes(0);
-    put_x(0);
-    put_sums(0);
-    const int stages = g.blocks * PLANES;
-    for (int stage = 0, b = 0, q = 0; stage < stages; ++stage) {
-        if (q == 0) {
+    if (first < end) {
+        fetch_x(first);
+        fetch_sums(first);
+        fetch_codes(first);
+        put_x(0);
+        put_sums(0);
+    }
+    for (int stage = first, half = 0; stage < end; ++stage, half ^= 1) {
 #pragma unroll
-            for (int j = 0; j < NC; ++j)
-                w[j] = wn[j];
-            fetch_meta(b);      // wanted when the first unit ends
-        }
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int s = 0; s < StageSteps; ++s)
+                w[j][s] = wn[j][s];
+        fetch_meta(stage);      // wanted when the first unit ends
         __syncthreads();        // this stage's tile is whole, and nobody reads the other any more
-        const int half = stage & 1;
-        const int bq = b, qq = q;
-        if (++q == PLANES) {
-            q = 0;
-            ++b;
+        if (stage + 1 < end) {
+            fetch_x(stage + 1);
+            fetch_sums(stage + 1);
+            fetch_codes(stage + 1);
         }
-        if (stage + 1 < stages) {
-            fetch_x(b, q);
-            if (q == 0) {
-                fetch_sums(b);
-                fetch_codes(b);
-            }
-        }
-        // the sums of a unit are scaled when it ends; the pieces of one fp32 x share the sum of x, which is taken off once
-        const bool last = qq == PLANES - 1;
 #pragma clang loop unroll(disable)
-        for (int u = 0; u < UNITS; ++u) {       // (unrolled, smaller units would need more registers than there are)
+        for (int u = 0; u < Loops; ++u) {       // (unrolled, smaller units would need more registers than there are)
 #pragma unroll
-            for (int i = 0; i < Steps; ++i) {
-                const int s = u * Steps + i;
-                u32x4 a[4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    a[t] = *reinterpret_cast<const u32x4*>(tile[half] + (t * 16 + c) * 256 + (((s * 4 + kb) ^ c) * 16));
+            for (int i = 0; i < LoopSteps; ++i) {
+                const int s = u * LoopSteps + i;
+                u32x4 wide[NC];
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
-                    const uint32_t word = UNITS == 1 ? w[j][i] : UNITS == 2 ? (u ? w[j][i + 2] : w[j][i])
-                                                     : u == 0 ? w[j][0] : u == 1 ? w[j][1] : u == 2 ? w[j][2] : w[j][3];
-                    const u32x4 wide = widened<T>(word);
+                    uint32_t word = w[j][i];
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        acc[t][j] = product<T>(a[t], wide, acc[t][j]);
+                    for (int k = 1; k < Loops; ++k)
+                        word = u == k ? w[j][k * LoopSteps + i] : word;
+                    wide[j] = widened<T>(word);
+                }
+#pragma unroll
+                for (int q = 0; q < PLANES; ++q) {
+                    u32x4 a[RT];
+#pragma unroll
+                    for (int t = 0; t < RT; ++t)
+                        a[t] = *reinterpret_cast<const u32x4*>(tile[half] + (t * 16 + c) * RowBytes +
+                                                               place_of(c, (q * StageSteps + s) * 4 + kb) * 16);
+#pragma unroll
+                    for (int j = 0; j < NC; ++j)
+#pragma unroll
+                        for (int t = 0; t < RT; ++t)
+                            acc[t][j] = product<T>(a[t], wide[j], acc[t][j]);
                 }
             }
-            if (last || UNITS > 1) {
-                f32x4 xs[4];
+            // the sums of a unit are scaled when it ends
+            if (StageSteps >= STEPS || (stage & 1)) {
+                f32x4 xs[RT];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    xs[t] = *reinterpret_cast<const f32x4*>(&sums[bq & 1][u][t * 16 + kb * 4]);
-                    if (PLANES > 1 && !last)
-                        xs[t] = f32x4{0, 0, 0, 0};
-                }
+                for (int t = 0; t < RT; ++t)
+                    xs[t] = *reinterpret_cast<const f32x4*>(&sums[half][u][t * 16 + kb * 4]);
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
-                    const uint32_t word = UNITS == 1 ? mt[j][0] : UNITS == 2 ? (u ? mt[j][UNITS - 1] : mt[j][0])
-                                                     : u == 0 ? mt[j][0] : u == 1 ? mt[j][1 % UNITS] : u == 2 ? mt[j][2 % UNITS] : mt[j][3 % UNITS];
+                    uint32_t word = mt[j][0];
+#pragma unroll
+                    for (int k = 1; k < Loops; ++k)
+                        word = u == k ? mt[j][k] : word;
                     const float scale = __uint_as_float(word & ~15u);
                     const float offset = -(16.0f + (float)(word & 15u));
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
+                    for (int t = 0; t < RT; ++t) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             total[t][j][e] = fmaf(scale, fmaf(offset, xs[t][e], acc[t][j][e]), total[t][j][e]);
@@ -292,10 +321,9 @@ q4_gemm_kernel(GemmArgs g)
                 }
             }
         }
-        if (stage + 1 < stages) {
+        if (stage + 1 < end) {
             put_x(half ^ 1);
-            if (q == 0)
-                put_sums(b);
+            put_sums(half ^ 1);
         }
     }
 
@@ -304,67 +332,125 @@ q4_gemm_kernel(GemmArgs g)
         const int col = (tile0 + j) * 16 + c;
         if (col >= g.N)
             continue;
-        const float bias = g.bias ? g.bias[col] : 0.0f;
+        const float bias = g.bias && g.splits == 1 ? g.bias[col] : 0.0f;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < RT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int row = t * 16 + kb * 4 + e;
-                if (row < rows_here)
+                if (row >= rows_here)
+                    continue;
+                if (g.splits > 1)
+                    g.partial[((size_t)blockIdx.y * g.M + m0 + row) * g.partial_ld + col] = total[t][j][e];
+                else
                     store_result<OUT>(g.y, (size_t)(m0 + row) * g.ldy + col, total[t][j][e] + bias);
             }
     }
 }
 
-template <ElementType T, int PLANES, ElementType OUT, int UNITS>
-void run_units(GemmArgs& g, hipStream_t stream)
+// The ranges of K added up in order.
+template <ElementType OUT>
+__global__ void __launch_bounds__(256)
+q4_gemm_reduce_kernel(const float* __restrict__ partial, size_t partial_ld, int splits, const float* __restrict__ bias,
+                      void* __restrict__ y, size_t ldy, int M, int N)
 {
-    g.tiles_m = (g.M + kRows - 1) / kRows;
-    g.tiles_n = (g.tiles + 15) / 16;
-    if (g.tiles_m * g.tiles_n >= 2 * machine().cus) {
-        q4_gemm_kernel<T, PLANES, OUT, 4, UNITS><<<g.tiles_m * g.tiles_n, 256, 0, stream>>>(g);
-    } else {
-        g.tiles_n = (g.tiles + 7) / 8;
-        q4_gemm_kernel<T, PLANES, OUT, 2, UNITS><<<g.tiles_m * g.tiles_n, 256, 0, stream>>>(g);
-    }
+    const int col = (blockIdx.y * 256 + threadIdx.x) * 4, row = blockIdx.x;
+    if (col >= N)
+        return;
+    f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s)
+        sum += *reinterpret_cast<const f32x4*>(partial + ((size_t)s * M + row) * partial_ld + col);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (col + e < N)
+            store_result<OUT>(y, (size_t)row * ldy + col + e, sum[e] + (bias ? bias[col + e] : 0.0f));
+}
+
+template <ElementType T, int PLANES, ElementType OUT, int STEPS>
+void run_steps(const GemmArgs& g, int row_tiles, int column_tiles, hipStream_t stream)
+{
+    const dim3 grid(g.tiles_m * g.tiles_n, g.splits);
+    if (row_tiles == 1)
+        q4_gemm_kernel<T, PLANES, OUT, 1, 2, STEPS><<<grid, 256, 0, stream>>>(g);
+    else if (row_tiles == 2)
+        q4_gemm_kernel<T, PLANES, OUT, 2, 2, STEPS><<<grid, 256, 0, stream>>>(g);
+    else if (column_tiles == 2)
+        q4_gemm_kernel<T, PLANES, OUT, 4, 2, STEPS><<<grid, 256, 0, stream>>>(g);
+    else
+        q4_gemm_kernel<T, PLANES, OUT, 4, 4, STEPS><<<grid, 256, 0, stream>>>(g);
+}
+
+// How a product is cut: a workgroup's row tiles and column tiles (of a wave), and the ranges of K.
+struct GemmCut {
+    int row_tiles, column_tiles, tiles_m, tiles_n, splits;
+};
+GemmCut gemm_cut(int M, int tiles, int blocks)
+{
+    GemmCut c;
+    const int cus = machine().cus;
+    c.row_tiles = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    c.tiles_m = (M + 16 * c.row_tiles - 1) / (16 * c.row_tiles);
+    c.column_tiles = c.row_tiles == 4 && c.tiles_m * ((tiles + 15) / 16) >= 2 * cus ? 4 : 2;
+    c.tiles_n = (tiles + 4 * c.column_tiles - 1) / (4 * c.column_tiles);
+    // two workgroups to a compute unit, as long as each has two blocks of K
+    const long long groups = (long long)c.tiles_m * c.tiles_n;
+    long long splits = (2 * cus + groups - 1) / groups;
+    if (splits > blocks / 2)
+        splits = blocks / 2;
+    c.splits = splits < 1 || groups >= 2 * cus ? 1 : (int)splits;
+    return c;
 }
 
 template <ElementType T, int PLANES, ElementType OUT>
-void run_gemm(GemmArgs& g, hipStream_t stream)
+void run_gemm(GemmArgs& g, const GemmCut& c, hipStream_t stream)
 {
+    g.tiles_m = c.tiles_m;
+    g.tiles_n = c.tiles_n;
+    g.splits = c.splits;
     if (g.unit == 128)
-        run_units<T, PLANES, OUT, 1>(g, stream);
+        run_steps<T, PLANES, OUT, 4>(g, c.row_tiles, c.column_tiles, stream);
     else if (g.unit == 64)
-        run_units<T, PLANES, OUT, 2>(g, stream);
+        run_steps<T, PLANES, OUT, 2>(g, c.row_tiles, c.column_tiles, stream);
     else
-        run_units<T, PLANES, OUT, 4>(g, stream);
+        run_steps<T, PLANES, OUT, 1>(g, c.row_tiles, c.column_tiles, stream);
+    if (c.splits > 1)
+        q4_gemm_reduce_kernel<OUT><<<dim3(g.M, (g.N + 1023) / 1024), 256, 0, stream>>>(g.partial, g.partial_ld, g.splits, g.bias, g.y,
+                                                                                       g.ldy, g.M, g.N);
 }
 
 size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
 } // namespace
 
-// What lies where in the workspace (bytes): the densified codes, the sums, the pieces of x.
+// What lies where in the workspace (bytes): the densified codes, the sums, the pieces of x, the ranges' results.
 struct GemmSpace {
-    size_t codes, sums, planes, bytes;
+    size_t codes, sums, planes, partial, bytes;
 };
-static GemmSpace gemm_space(const Q4Shape& p, int M, ElementType type, bool codes, bool product, bool planes)
+static GemmSpace gemm_space(const Q4Shape& p, int M, ElementType type, bool codes, bool product)
 {
     const size_t blocks = ((size_t)p.K + 127) / 128;
     GemmSpace s;
     s.codes = 0;
     s.sums = codes ? p.tiles * blocks * 1024 : 0;
-    s.planes = s.sums + (product ? round_up(blocks * 4 * round_up(M, 4) * sizeof(float), 256) : 0);
-    s.bytes = s.planes + (product && planes ? (type == kF32 ? 3 : 1) * (size_t)M * blocks * 256 : 0);
+    s.planes = s.sums;
+    s.partial = s.sums;
+    s.bytes = s.sums;
+    if (product) {
+        const GemmCut c = gemm_cut(M, p.tiles, (int)blocks);
+        s.planes = s.sums + round_up(blocks * 4 * round_up(M, 4) * sizeof(float), 256);
+        s.partial = s.planes + (type == kF32 ? 3 : 1) * (size_t)M * blocks * 256;
+        s.bytes = s.partial + (c.splits > 1 ? (size_t)c.splits * M * round_up(p.N, 4) * sizeof(float) : 0);
+    }
     return s;
 }
 
-bool q4_uses_gemm(const Q4Shape&, int M) { return M > 64; }
-bool q4_densifies(const Q4Shape& p, int M) { return p.m > 1 && M > 16; }
+bool q4_uses_gemm(const Q4Shape&, int M) { return M > 4; }
+bool q4_densifies(const Q4Shape& p, int M) { return p.m > 1 && M > 4; }
 
 size_t q4_workspace_bytes(const Q4Shape& p, int M, ElementType type)
 {
-    return gemm_space(p, M, type, q4_densifies(p, M), q4_uses_gemm(p, M), true).bytes;
+    return gemm_space(p, M, type, q4_densifies(p, M), q4_uses_gemm(p, M)).bytes;
 }
 
 hipError_t launch_q4_densify(const Q4LinearArgs& a, uint32_t* out)
@@ -377,7 +463,8 @@ hipError_t launch_q4_densify(const Q4LinearArgs& a, uint32_t* out)
 // `a` is dense by now (q4_linear.hip).
 hipError_t launch_q4_gemm(const Q4LinearArgs& a, ElementType type, bool densified, void* workspace)
 {
-    const GemmSpace s = gemm_space(a.p, a.M, type, densified, true, true);
+    const GemmSpace s = gemm_space(a.p, a.M, type, densified, true);
+    const GemmCut c = gemm_cut(a.M, a.p.tiles, a.p.blocks);
     char* const base = static_cast<char*>(workspace);
     const int Kp = a.p.blocks * 128;
     GemmArgs g;
@@ -394,9 +481,11 @@ hipError_t launch_q4_gemm(const Q4LinearArgs& a, ElementType type, bool densifie
     g.Kx = Kp;
     g.blocks = a.p.blocks;
     g.tiles = a.p.tiles;
+    g.partial = reinterpret_cast<float*>(base + s.partial);
+    g.partial_ld = round_up(a.p.N, 4);
     uint16_t* const planes = reinterpret_cast<uint16_t*>(base + s.planes);
     const dim3 grid((a.M + 3) / 4, (Kp + 511) / 512);
-    // x as it is: 16-bit elements, rows of whole blocks on 16-byte boundaries, 64 of them within 2 GiB
+    // x as it is: 16-bit elements, rows of whole blocks on 16-byte boundaries, 64 of them within 1 GiB
     const bool as_is = type != kF32 && a.p.K == Kp && a.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15u) == 0 &&
                        a.ldx < (1u << 23);
     float* const sums = const_cast<float*>(g.sums);
@@ -410,8 +499,8 @@ hipError_t launch_q4_gemm(const Q4LinearArgs& a, ElementType type, bool densifie
             q4_prepare_x_kernel<kF16, 0><<<grid, 256, 0, a.stream>>>(a.x, a.ldx, a.M, a.p.K, Kp, g.unit, nullptr, sums, g.sums_ld);
     } else {
         g.x = planes;
-        g.ldx = Kp;
-        g.plane = (size_t)a.M * Kp;
+        g.ldx = type == kF32 ? 3 * (size_t)Kp : Kp;
+        g.plane = Kp;
         if (type == kF32)
             q4_prepare_x_kernel<kF32, 3><<<grid, 256, 0, a.stream>>>(a.x, a.ldx, a.M, a.p.K, Kp, g.unit, planes, sums, g.sums_ld);
         else if (type == kBF16)
@@ -420,11 +509,11 @@ hipError_t launch_q4_gemm(const Q4LinearArgs& a, ElementType type, bool densifie
             q4_prepare_x_kernel<kF16, 1><<<grid, 256, 0, a.stream>>>(a.x, a.ldx, a.M, a.p.K, Kp, g.unit, planes, sums, g.sums_ld);
     }
     if (type == kF32)
-        run_gemm<kBF16, 3, kF32>(g, a.stream);
+        run_gemm<kBF16, 3, kF32>(g, c, a.stream);
     else if (type == kBF16)
-        run_gemm<kBF16, 1, kBF16>(g, a.stream);
+        run_gemm<kBF16, 1, kBF16>(g, c, a.stream);
     else
-        run_gemm<kF16, 1, kF16>(g, a.stream);
+        run_gemm<kF16, 1, kF16>(g, c, a.stream);
     return hipGetLastError();
 }
 
