@@ -369,11 +369,11 @@ int nmspmm_q4_pack_device(const uint8_t* d_codes, const float* d_scales, const u
 /* The operand as the dense fp32 matrix dB[K][N], zeros where rows were not kept (exact). */
 int nmspmm_q4_expand_device(const nmspmm_q4_operand* op, float* dB, void* stream);
 
-/* y[M][N] = x[M][K] B + bias: rows of x are ldx elements apart (ldx >= K), rows of y ldy (>= N), both of
+/* y[M][N] = x[M][K] B + bias: rows of x are ldx elements apart (K to 2^24), rows of y ldy (N to 2^24), both of
  * `type`; sums in fp32, one rounding at the end.  M == 0 does nothing.  fp32 activations are multiplied
  * exactly (three bf16 pieces each), so the result is as near as an fp32 product's.  A row of x that
  * holds an infinity or a NaN, or magnitudes beyond 2^100, gives a row of NaN.  x and y must not overlap.
- * The workspace (16-byte aligned) holds what nmspmm_q4_workspace_bytes says, which is 0 for up to 4 rows (it may be NULL
+ * The workspace (16-byte aligned) holds what nmspmm_q4_workspace_bytes says, which is 0 for up to 8 rows (it may be NULL
  * then).  Calls that may overlap in time take workspaces of their own;
  * nothing is kept in one from call to call.  No library state: any streams and threads; may be captured into a HIP graph.
  * Results repeat bit for bit. */

@@ -141,7 +141,7 @@ int nmspmm_q4_linear(const nmspmm_q4_operand* op, const void* x, long long ldx, 
         return st;
     if (type != NMSPMM_F32 && type != NMSPMM_BF16 && type != NMSPMM_F16)
         return NMSPMM_ERR_BAD_PATTERN;
-    if (M < 0 || M > (1 << 24) || ldx < p.K || ldy < p.N)
+    if (M < 0 || M > (1 << 24) || ldx < p.K || ldy < p.N || ldx > (1 << 24) || ldy > (1 << 24))
         return NMSPMM_ERR_BAD_SHAPE;
     if (M == 0)
         return NMSPMM_OK;

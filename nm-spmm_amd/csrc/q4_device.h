@@ -19,15 +19,23 @@ __device__ inline f32x4 product(u32x4 a, u32x4 b, f32x4 c)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// 16.0 twice, kept in a vector register: an instruction takes one scalar, and mask-and-or needs this and the mask (with both
+// as constants the compiler makes a mask and an or of it: half as many instructions again).
+template <ElementType T>
+__device__ inline uint32_t sixteens()
+{
+    uint32_t one = T == kF16 ? 0x4c004c00u : 0x41804180u;
+    asm("" : "+v"(one));
+    return one;
+}
+
 // Eight codes -> eight operand elements 16 + code.
 template <ElementType T>
-__device__ inline u32x4 widened(uint32_t w)
+__device__ inline u32x4 widened(uint32_t w, uint32_t one)
 {
-    if (T == kF16) {
-        const uint32_t mask = 0x03c003c0u, one = 0x4c004c00u;
+    const uint32_t mask = T == kF16 ? 0x03c003c0u : 0x00780078u;
+    if (T == kF16)
         return u32x4{((w << 6) & mask) | one, ((w << 2) & mask) | one, ((w >> 2) & mask) | one, ((w >> 6) & mask) | one};
-    }
-    const uint32_t mask = 0x00780078u, one = 0x41804180u;
     return u32x4{((w << 3) & mask) | one, ((w >> 1) & mask) | one, ((w >> 5) & mask) | one, ((w >> 9) & mask) | one};
 }
 
@@ -40,6 +48,17 @@ __device__ inline void store_result(void* y, size_t at, float v)
         static_cast<uint16_t*>(y)[at] = __builtin_bit_cast(uint16_t, (__bf16)v);
     else
         static_cast<uint16_t*>(y)[at] = __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+
+// The same through a descriptor, at a byte offset from its base; beyond its bounds nothing is stored.
+template <ElementType T>
+__device__ inline void store_bounded(__amdgpu_buffer_rsrc_t r, uint32_t offset, float v)
+{
+    if (T == kF32)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, (int)offset, 0, 0);
+    else
+        __builtin_amdgcn_raw_buffer_store_b16(T == kBF16 ? __builtin_bit_cast(uint16_t, (__bf16)v) : __builtin_bit_cast(uint16_t, (_Float16)v),
+                                              r, (int)offset, 0, 0);
 }
 
 } // namespace nmspmm

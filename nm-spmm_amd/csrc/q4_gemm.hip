@@ -81,6 +81,7 @@ q4_prepare_x_kernel(const void* __restrict__ x_, size_t ldx, int M, int K, int K
 
 // ---- a sparse operand's codes as those of a dense one: the zero point where no row was kept ----------------
 
+template <int KEPT>     // kept rows that can lie among eight dense ones: those of their windows, or of the one they are part of
 __global__ void __launch_bounds__(256)
 q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict__ meta, const uint8_t* __restrict__ rows,
                   Q4Shape p, int dense_blocks, uint32_t* __restrict__ out)
@@ -93,27 +94,22 @@ q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict
     u32x4 word;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        const int d0 = block * 128 + s * 32 + kb * 8;       // eight dense rows
-        // the kept rows that can lie among them: those of their windows, or of the one window they are a part of
-        const int count = p.m > 8 ? p.n : 8 / p.m * p.n;
-        const int r0 = d0 / p.m * p.n;                      // a multiple of count: all in one word
-        const int b = r0 >> 7, step = (r0 >> 5) & 3, part = (r0 >> 3) & 3;
-        uint32_t dense = 0x88888888u;
-        if (d0 < p.K) {
-            const size_t at = (size_t)tile * p.blocks + b;
-            const uint32_t zero = meta[(at * 16 + c) * per + step * per / 4] & 15u;
-            dense = zero * 0x11111111u;
-            const uint32_t packed = codes[(at * 64 + part * 16 + c) * 4 + step];
-            const uint8_t* const off = rows + (size_t)(tile >> 1) * p.blocks * 128 + r0;
-            const int base = (r0 >> 5) * p.span - d0;
-            for (int i = 0; i < count; ++i) {
-                const int e = (r0 & 7) + i;
-                const int d = base + off[i];                // 0..7 if it is among the eight
-                const uint32_t q = (packed >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u;
-                const int to = 4 * ((d >> 1) + 4 * (d & 1));
-                if (d >= 0 && d < 8 && r0 + i < p.W)
-                    dense = (dense & ~(15u << to)) | q << to;
-            }
+        const int d0 = min(block * 128 + s * 32 + kb * 8, (p.K - 1) & ~7);  // eight dense rows (of padding: anything, x is zero there)
+        const int r0 = d0 / p.m * p.n;                                      // a multiple of KEPT: all in one word
+        const size_t at = (size_t)tile * p.blocks + (r0 >> 7);
+        const uint32_t zero = meta[(at * 16 + c) * per + ((r0 >> 5) & 3) * per / 4] & 15u;
+        const uint32_t packed = codes[(at * 64 + ((r0 >> 3) & 3) * 16 + c) * 4 + ((r0 >> 5) & 3)];
+        const uint2 eight = *reinterpret_cast<const uint2*>(rows + (size_t)(tile >> 1) * p.blocks * 128 + (r0 & ~7));
+        const int base = (r0 >> 5) * p.span - d0;
+        uint32_t dense = zero * 0x11111111u;
+#pragma unroll
+        for (int i = 0; i < KEPT; ++i) {
+            const int e = (r0 & 7) + i;
+            const uint32_t off = ((e < 4 ? eight.x : eight.y) >> (8 * (e & 3))) & 255u;
+            const uint32_t d = (uint32_t)(base + (int)off);                 // 0..7 if it is among the eight
+            // what changes from the zero point to the code, put at its place (nibble of row d: 4 (d / 2 + 4 (d % 2)))
+            const uint32_t change = ((packed >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) ^ zero;
+            dense ^= d < 8u && r0 + i < p.W ? change << (2 * (d & 6) + 16 * (d & 1)) : 0u;
         }
         word[s] = dense;
     }
@@ -177,7 +173,7 @@ q4_gemm_kernel(GemmArgs g)
     for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int j = 0; j < NC; ++j)
-            acc[t][j] = total[t][j] = f32x4{0, 0, 0, 0};
+            total[t][j] = f32x4{0, 0, 0, 0};
 
     // Where piece q of row r lies in a row of the tile: swapped so that the sixteen rows of a read start in different banks.
     auto place_of = [&](int r, int q) {
@@ -196,6 +192,7 @@ q4_gemm_kernel(GemmArgs g)
     }
     // Through registers and not straight into LDS: behind such a load the compiler lets every LDS read wait for it.
     u32x4 xr[Mine];
+    const uint32_t one = sixteens<T>();
     uint32_t sr = 0;
     auto fetch_x = [&](int stage) {
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
@@ -222,7 +219,7 @@ q4_gemm_kernel(GemmArgs g)
         if (wave < Loops && lane < Rows)
             sums[half][wave][lane] = __uint_as_float(sr);
     };
-    uint32_t w[NC][StageSteps], wn[NC][StageSteps], mt[NC][Loops];
+    uint32_t w[NC][StageSteps], wn[NC][StageSteps], mt[NC][Loops], mn[NC][Loops];
     auto fetch_codes = [&](int stage) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
@@ -246,13 +243,14 @@ q4_gemm_kernel(GemmArgs g)
         for (int j = 0; j < NC; ++j)
 #pragma unroll
             for (int u = 0; u < Loops; ++u)
-                mt[j][u] = g.meta.word(min(tile0 + j, g.tiles - 1), (stage * StageSteps + u * LoopSteps) * 32, c);
+                mn[j][u] = g.meta.word(min(tile0 + j, g.tiles - 1), (stage * StageSteps + u * LoopSteps) * 32, c);
     };
 
     if (first < end) {
         fetch_x(first);
         fetch_sums(first);
         fetch_codes(first);
+        fetch_meta(first);
         put_x(0);
         put_sums(0);
     }
@@ -262,15 +260,40 @@ q4_gemm_kernel(GemmArgs g)
 #pragma unroll
             for (int s = 0; s < StageSteps; ++s)
                 w[j][s] = wn[j][s];
-        fetch_meta(stage);      // wanted when the first unit ends
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int u = 0; u < Loops; ++u)
+                mt[j][u] = mn[j][u];
         __syncthreads();        // this stage's tile is whole, and nobody reads the other any more
         if (stage + 1 < end) {
             fetch_x(stage + 1);
             fetch_sums(stage + 1);
             fetch_codes(stage + 1);
+            fetch_meta(stage + 1);
         }
 #pragma clang loop unroll(disable)
         for (int u = 0; u < Loops; ++u) {       // (unrolled, smaller units would need more registers than there are)
+            // a unit's sums start from what its offset takes off, - (16 + zero) times the sum of x
+            if (StageSteps >= STEPS || !(stage & 1)) {
+                f32x4 xs[RT];
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                    xs[t] = *reinterpret_cast<const f32x4*>(&sums[half][u][t * 16 + kb * 4]);
+#pragma unroll
+                for (int j = 0; j < NC; ++j) {
+                    uint32_t word = mt[j][0];
+#pragma unroll
+                    for (int k = 1; k < Loops; ++k)
+                        word = u == k ? mt[j][k] : word;
+                    const float offset = -(16.0f + (float)(word & 15u));
+#pragma unroll
+                    for (int t = 0; t < RT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[t][j][e] = offset * xs[t][e];
+                }
+            }
 #pragma unroll
             for (int i = 0; i < LoopSteps; ++i) {
                 const int s = u * LoopSteps + i;
@@ -281,7 +304,7 @@ q4_gemm_kernel(GemmArgs g)
 #pragma unroll
                     for (int k = 1; k < Loops; ++k)
                         word = u == k ? w[j][k * LoopSteps + i] : word;
-                    wide[j] = widened<T>(word);
+                    wide[j] = widened<T>(word, one);
                 }
 #pragma unroll
                 for (int q = 0; q < PLANES; ++q) {
@@ -297,12 +320,8 @@ q4_gemm_kernel(GemmArgs g)
                             acc[t][j] = product<T>(a[t], wide[j], acc[t][j]);
                 }
             }
-            // the sums of a unit are scaled when it ends
+            // and are scaled when it ends
             if (StageSteps >= STEPS || (stage & 1)) {
-                f32x4 xs[RT];
-#pragma unroll
-                for (int t = 0; t < RT; ++t)
-                    xs[t] = *reinterpret_cast<const f32x4*>(&sums[half][u][t * 16 + kb * 4]);
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
                     uint32_t word = mt[j][0];
@@ -310,14 +329,11 @@ q4_gemm_kernel(GemmArgs g)
                     for (int k = 1; k < Loops; ++k)
                         word = u == k ? mt[j][k] : word;
                     const float scale = __uint_as_float(word & ~15u);
-                    const float offset = -(16.0f + (float)(word & 15u));
 #pragma unroll
-                    for (int t = 0; t < RT; ++t) {
+                    for (int t = 0; t < RT; ++t)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            total[t][j][e] = fmaf(scale, fmaf(offset, xs[t][e], acc[t][j][e]), total[t][j][e]);
-                        acc[t][j] = f32x4{0, 0, 0, 0};
-                    }
+                            total[t][j][e] = fmaf(scale, acc[t][j][e], total[t][j][e]);
                 }
             }
         }
@@ -327,24 +343,30 @@ q4_gemm_kernel(GemmArgs g)
         }
     }
 
+    // rows beyond M and columns beyond N lie outside the descriptors
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-        const int col = (tile0 + j) * 16 + c;
-        if (col >= g.N)
-            continue;
-        const float bias = g.bias && g.splits == 1 ? g.bias[col] : 0.0f;
+    for (int t = 0; t < RT; ++t) {
+        const int rows = min(16, rows_here - t * 16);
+        if (rows <= 0)
+            break;
+        const size_t ld = g.splits > 1 ? g.partial_ld : g.ldy;
+        const size_t size = g.splits > 1 || OUT == kF32 ? 4 : 2;
+        char* const base = g.splits > 1 ? reinterpret_cast<char*>(g.partial + ((size_t)blockIdx.y * g.M + m0 + t * 16) * ld)
+                                        : static_cast<char*>(g.y) + (size_t)(m0 + t * 16) * ld * size;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(base, 0, (int)(((rows - 1) * ld + g.N) * size), 0x00020000);
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+        for (int j = 0; j < NC; ++j) {
+            const int col = (tile0 + j) * 16 + c;
+            const float bias = g.bias && g.splits == 1 && col < g.N ? g.bias[col] : 0.0f;
+            const uint32_t at = col < g.N ? (uint32_t)((kb * 4 * ld + col) * size) : 0x80000000u;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int row = t * 16 + kb * 4 + e;
-                if (row >= rows_here)
-                    continue;
                 if (g.splits > 1)
-                    g.partial[((size_t)blockIdx.y * g.M + m0 + row) * g.partial_ld + col] = total[t][j][e];
+                    store_bounded<kF32>(r, at + (uint32_t)(e * ld * size), total[t][j][e]);
                 else
-                    store_result<OUT>(g.y, (size_t)(m0 + row) * g.ldy + col, total[t][j][e] + bias);
+                    store_bounded<OUT>(r, at + (uint32_t)(e * ld * size), total[t][j][e] + bias);
             }
+        }
     }
 }
 
@@ -445,18 +467,21 @@ static GemmSpace gemm_space(const Q4Shape& p, int M, ElementType type, bool code
     return s;
 }
 
-bool q4_uses_gemm(const Q4Shape&, int M) { return M > 4; }
-bool q4_densifies(const Q4Shape& p, int M) { return p.m > 1 && M > 4; }
+bool q4_densifies(const Q4Shape& p, int M) { return p.m > 1 && M > 16; }
 
 size_t q4_workspace_bytes(const Q4Shape& p, int M, ElementType type)
 {
-    return gemm_space(p, M, type, q4_densifies(p, M), q4_uses_gemm(p, M)).bytes;
+    // (whether 9 to 16 rows of 16-bit elements are aligned is not known here)
+    return gemm_space(p, M, type, q4_densifies(p, M), M > (type == kF32 || p.m > 1 ? 16 : 8)).bytes;
 }
 
 hipError_t launch_q4_densify(const Q4LinearArgs& a, uint32_t* out)
 {
     const int blocks = (a.p.K + 127) / 128;
-    q4_densify_kernel<<<dim3(blocks, (a.p.tiles + 3) / 4), 256, 0, a.stream>>>(a.codes, a.meta.words, a.rows, a.p, blocks, out);
+    const dim3 grid(blocks, (a.p.tiles + 3) / 4);
+    const int kept = a.p.m > 8 ? a.p.n : 8 / a.p.m * a.p.n;
+    auto kernel = kept == 1 ? q4_densify_kernel<1> : kept == 2 ? q4_densify_kernel<2> : kept == 4 ? q4_densify_kernel<4> : q4_densify_kernel<8>;
+    kernel<<<grid, 256, 0, a.stream>>>(a.codes, a.meta.words, a.rows, a.p, blocks, out);
     return hipGetLastError();
 }
 

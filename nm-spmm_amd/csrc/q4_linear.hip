@@ -17,6 +17,7 @@ namespace nmspmm {
 namespace {
 
 constexpr int kMaxWaves = 16;
+constexpr size_t kMostLds = 131072;
 constexpr int kRowPitch = 136;      // 16-bit elements between staged rows: 128 and 16 bytes, so that the sixteen
                                     // rows of a 128-bit LDS read start in different banks
 
@@ -33,8 +34,11 @@ __device__ inline __amdgpu_buffer_rsrc_t window(const void* base, size_t bytes)
 // and add up their sums in LDS at the end, in wave order.  A block costs about 60 vector instructions a tile, which is what bounds
 // the kernel beside the launch: addresses are scalars, ends are left to the descriptors' bounds, groups are unrolled.
 // MX: rows of x the instance has registers for; UNITS: scaled groups in a block; the next DEPTH blocks are on their way.
+// What an instance needs registers for decides how many waves it runs with.
+constexpr int most_waves(int RT, int MX) { return MX > 8 || (RT > 1 && MX == 1) ? kMaxWaves / 2 : kMaxWaves; }
+
 template <ElementType T, Source SRC, int RT, int NC, int MX, int UNITS>
-__global__ void __launch_bounds__(kMaxWaves * 64)
+__global__ void __launch_bounds__(most_waves(RT, MX) * 64)
 q4_rows_product_kernel(const void* __restrict__ x_, size_t ldx, const uint32_t* __restrict__ codes, Q4Meta meta,
                        const uint8_t* __restrict__ rows, const float* __restrict__ bias, void* __restrict__ y, size_t ldy, int M,
                        Q4Shape p, bool pairs)
@@ -59,6 +63,7 @@ q4_rows_product_kernel(const void* __restrict__ x_, size_t ldx, const uint32_t* 
             total[t][j] = f32x4{0, 0, 0, 0};
     const uint32_t unit = T == kF16 ? 0x3c003c00u : 0x3f803f80u;
     const u32x4 unit8 = u32x4{unit, unit, unit, unit};
+    const uint32_t sixteen = sixteens<T>();
 
     // this lane's place in x: its row and first element of a step, or its two kept rows of a block
     const __amdgpu_buffer_rsrc_t all = window(x_, ((size_t)(M - 1) * ldx + p.K) * Size);
@@ -179,7 +184,7 @@ q4_rows_product_kernel(const void* __restrict__ x_, size_t ldx, const uint32_t* 
                     ones[t] = product<T>(xa[t][s], unit8, i ? ones[t] : f32x4{0, 0, 0, 0});
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
-                    const u32x4 wide = widened<T>(n.w[j][s]);
+                    const u32x4 wide = widened<T>(n.w[j][s], sixteen);
 #pragma unroll
                     for (int t = 0; t < RT; ++t)
                         acc[t][j] = product<T>(xa[t][s], wide, i ? acc[t][j] : f32x4{0, 0, 0, 0});
@@ -257,12 +262,23 @@ hipError_t launch_rows(const Q4LinearArgs& a, bool pairs)
     constexpr int Chunk = RT * (T == kF32 ? 4 : 16);
     // one workgroup to a compute unit: sixteen waves each; more workgroups than that: eight (measured, us with 8 / 16 waves:
     // 4096 x 14336 dense 8.7 / 9.3, 2:4 5.7 / 7.0 at one row; 8192 x 8192 9.9 / 8.4, 11008 x 4096 9.3 / 8.0)
-    const int most = a.p.tiles / NC > machine().cus ? kMaxWaves / 2 : kMaxWaves;
-    const int waves = a.p.blocks < most ? a.p.blocks : most;
-    const size_t staged = SRC == kDirect ? 0 : (size_t)waves * MX * (T == kF32 ? 3 : 1) * kRowPitch * 2;
-    const size_t sums = (size_t)waves * Chunk * NC * 16 * sizeof(float);
-    const size_t lds = staged > sums ? staged : sums;
-    q4_rows_product_kernel<T, SRC, RT, NC, MX, UNITS><<<a.p.tiles / NC, waves * 64, lds, a.stream>>>(
+    int most = a.p.tiles / NC > machine().cus ? kMaxWaves / 2 : kMaxWaves;
+    if (most > most_waves(RT, MX))
+        most = most_waves(RT, MX);
+    const size_t staged = SRC == kDirect ? 0 : (size_t)MX * (T == kF32 ? 3 : 1) * kRowPitch * 2;
+    const size_t sums = (size_t)Chunk * NC * 16 * sizeof(float);
+    const size_t each = staged > sums ? staged : sums;
+    int waves = a.p.blocks < most ? a.p.blocks : most;
+    if (each * waves > kMostLds)
+        waves = kMostLds / each;
+    const size_t lds = each * waves;
+    auto kernel = q4_rows_product_kernel<T, SRC, RT, NC, MX, UNITS>;
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess)
+            return e;
+    }
+    kernel<<<a.p.tiles / NC, waves * 64, lds, a.stream>>>(
         a.x, a.ldx, a.codes, a.meta, a.rows, a.bias, a.y, a.ldy, a.M, a.p, pairs);
     return hipGetLastError();
 }
@@ -283,15 +299,33 @@ hipError_t launch_units(const Q4LinearArgs& a, bool pairs)
 template <ElementType T, Source SRC>
 hipError_t launch_source(const Q4LinearArgs& a, bool pairs)
 {
-    if (SRC == kDirect)
-        return launch_units<T, kDirect, 1, 1>(a, pairs);
-    return a.M == 1 ? launch_units<T, SRC == kDirect ? kStaged : SRC, 1, 1>(a, pairs) : launch_units<T, SRC == kDirect ? kStaged : SRC, 1, 4>(a, pairs);
+    if constexpr (SRC == kDirect)
+        return a.M <= 16 ? launch_units<T, SRC, 1, 1>(a, pairs) : launch_units<T, SRC, 2, 1>(a, pairs);
+    else {
+        if (a.M == 1)
+            return launch_units<T, SRC, 1, 1>(a, pairs);
+        if (a.M <= 4)
+            return launch_units<T, SRC, 1, 4>(a, pairs);
+        if (a.M <= 8)
+            return launch_units<T, SRC, T == kF32 ? 2 : 1, 8>(a, pairs);
+        return launch_units<T, SRC, T == kF32 ? 4 : 1, 16>(a, pairs);
+    }
 }
 
 // x can be read as matrix operands where it lies
 bool direct(const Q4LinearArgs& a, ElementType type)
 {
     return type != kF32 && !a.rows && a.p.K % 128 == 0 && a.ldx % 8 == 0 && a.ldx < (1u << 24) && (reinterpret_cast<uintptr_t>(a.x) & 15u) == 0;
+}
+
+// Whether the kernel above takes the rows.  Measured against the other one (q4_gemm.hip), us at 4096 x 4096: as they lie, 16 / 32
+// rows 6.4 / 10.1 against 12 / 14.3 (11008 x 4096: 14 / 23.4 against 17.5 with 32); fp32, 8 / 16 rows 6.9 / 12.0 against 12.3 / 13.9;
+// 16-bit rows that are not aligned, 16 of them 27.9 against 12.
+bool few_rows(const Q4LinearArgs& a, ElementType type)
+{
+    if (direct(a, type))
+        return a.M <= 16 || (a.M <= 32 && a.p.blocks <= 48);
+    return a.M <= (type == kF32 || a.rows ? 16 : 8);
 }
 
 } // namespace
@@ -312,7 +346,7 @@ hipError_t launch_q4_linear(const Q4LinearArgs& given, ElementType type, void* w
         a.p.W = a.p.K;
         a.p.blocks = (a.p.K + 127) / 128;
     }
-    if (a.M > (direct(a, type) ? 16 : 4))
+    if (!few_rows(a, type))
         return launch_q4_gemm(a, type, densified, workspace);
     const size_t size = type == kF32 ? 4 : 2;
     const uintptr_t base = reinterpret_cast<uintptr_t>(a.x);

@@ -236,7 +236,7 @@ def _quant_linear(x, operand):
 
 def _launch_quant_linear(x, ldx, y, ldy, M, operand, device):
     type_, need, space = _TYPES[x.dtype], 0, None
-    if M > 4:       # below, no operand needs a workspace
+    if M > 8:       # below, no operand needs a workspace
         need = _nm.lib().nmspmm_q4_workspace_bytes(M, operand.K, operand.N, operand.n, operand.m, type_)
         if need:
             workspace = x.new_empty(need, dtype=torch.uint8)    # from torch's caching allocator, ordered on the stream

@@ -54,7 +54,7 @@ def test_refusals_of_the_other_arguments():
     assert L.nmspmm_q4_linear(dense, ctypes.c_void_p(0x10001), 256, FAKE, 64, 1, 1, None, 0, None) == 8
     many = nmspmm.q4_workspace_bytes(65, 256, 64, 1, 1, 0)
     assert many > 0
-    for rows in (1, 4):     # decoding takes no workspace
+    for rows in (1, 8):     # decoding takes no workspace
         assert nmspmm.q4_workspace_bytes(rows, 256, 64, 1, 1, 0) == 0 and nmspmm.q4_workspace_bytes(rows, 256, 64, 2, 4, 1) == 0
     for bad in ((0, 256, 64, 1, 1, 0), (-1, 256, 64, 1, 1, 0), (65, 256, 64, 1, 1, 3), (65, 0, 64, 1, 1, 0), (65, 256, 64, 3, 8, 0)):
         assert nmspmm.q4_workspace_bytes(*bad) == 0
