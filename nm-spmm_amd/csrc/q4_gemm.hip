@@ -118,6 +118,8 @@ q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict
 
 // ---- the product --------------------------------------------------------------------------------------------
 
+typedef __attribute__((address_space(3))) uint32_t lds_u32;
+
 struct GemmArgs {
     const uint16_t* x;      // rows ldx elements apart, their planes `plane`; 64 rows within 2 GiB
     size_t plane, ldx;
@@ -179,33 +181,25 @@ q4_gemm_kernel(GemmArgs g)
     auto place_of = [&](int r, int q) {
         return PLANES == 1 ? q ^ (r & 15) : (q & ~7) | ((q ^ (r >> 1)) & 7);
     };
-    uint32_t from[Mine], to[Mine];
+    // A wave brings 1 KB at a time straight into LDS, where lane l's piece lands at place l: lane and place fix row and piece.
+    uint32_t from[Mine];
 #pragma unroll
     for (int i = 0; i < Mine; ++i) {
-        const int n = i * 256 + threadIdx.x;
-        const int r = n / Pieces, q = n % Pieces;
-        // (a piece more than there are, or of a row beyond M: read as zero, and the former is not put down)
+        const int n = (i * 4 + wave) * 64 + lane;
+        const int r = n / Pieces, q = place_of(r, n % Pieces);     // (the swap is its own inverse)
         from[i] = (uint32_t)((q / (StageSteps * 4)) * g.plane * 2 + r * g.ldx * 2 + (q % (StageSteps * 4)) * 16);
         if (r >= rows_here)
-            from[i] = 0x80000000u;
-        to[i] = (uint32_t)(r * RowBytes + place_of(r, q) * 16);
+            from[i] = 0x80000000u;      // read as zero
     }
-    // Through registers and not straight into LDS: behind such a load the compiler lets every LDS read wait for it.
-    u32x4 xr[Mine];
-    const uint32_t one = sixteens<T>();
     uint32_t sr = 0;
-    auto fetch_x = [&](int stage) {
+    const uint32_t one = sixteens<T>();
+    auto fetch_x = [&](int stage, unsigned char* to) {
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint16_t*>(g.x + (size_t)m0 * g.ldx + stage * (StageSteps * 32)), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
         for (int i = 0; i < Mine; ++i)
-            xr[i] = __builtin_amdgcn_raw_buffer_load_b128(r, (int)from[i], 0, 0);
-    };
-    auto put_x = [&](int half) {
-#pragma unroll
-        for (int i = 0; i < Mine; ++i)
-            if (Rows * Pieces % 256 == 0 || i * 256 + (int)threadIdx.x < Rows * Pieces)
-                *reinterpret_cast<u32x4*>(tile[half] + to[i]) = xr[i];
+            if (Rows * Pieces % 256 == 0 || (i * 4 + wave) * 64 < Rows * Pieces)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_u32*)(to + (i * 4 + wave) * 1024), 16, (int)from[i], 0, 0, 0);
     };
     auto fetch_sums = [&](int stage) {
         if (wave < Loops) {
@@ -219,7 +213,7 @@ q4_gemm_kernel(GemmArgs g)
         if (wave < Loops && lane < Rows)
             sums[half][wave][lane] = __uint_as_float(sr);
     };
-    uint32_t w[NC][StageSteps], wn[NC][StageSteps], mt[NC][Loops], mn[NC][Loops];
+    uint32_t w[NC][StageSteps], wn[NC][StageSteps], mt[NC], mn[NC];
     auto fetch_codes = [&](int stage) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
@@ -238,55 +232,41 @@ q4_gemm_kernel(GemmArgs g)
             }
         }
     };
-    auto fetch_meta = [&](int stage) {
+    auto fetch_meta = [&](int step) {
 #pragma unroll
         for (int j = 0; j < NC; ++j)
-#pragma unroll
-            for (int u = 0; u < Loops; ++u)
-                mn[j][u] = g.meta.word(min(tile0 + j, g.tiles - 1), (stage * StageSteps + u * LoopSteps) * 32, c);
+            mn[j] = g.meta.word(min(tile0 + j, g.tiles - 1), step * 32, c);
     };
 
-    if (first < end) {
-        fetch_x(first);
-        fetch_sums(first);
-        fetch_codes(first);
-        fetch_meta(first);
-        put_x(0);
-        put_sums(0);
-    }
-    for (int stage = first, half = 0; stage < end; ++stage, half ^= 1) {
-#pragma unroll
-        for (int j = 0; j < NC; ++j)
-#pragma unroll
-            for (int s = 0; s < StageSteps; ++s)
-                w[j][s] = wn[j][s];
-#pragma unroll
-        for (int j = 0; j < NC; ++j)
-#pragma unroll
-            for (int u = 0; u < Loops; ++u)
-                mt[j][u] = mn[j][u];
-        __syncthreads();        // this stage's tile is whole, and nobody reads the other any more
+    // Declared not to overlap, so that the reads of this stage's tile do not wait for the next one's arrival.
+    auto multiply = [&](int stage, const unsigned char* __restrict__ now, const float* __restrict__ sums_now, unsigned char* __restrict__ next)
+        __attribute__((always_inline)) {
         if (stage + 1 < end) {
-            fetch_x(stage + 1);
+            fetch_x(stage + 1, next);
             fetch_sums(stage + 1);
             fetch_codes(stage + 1);
-            fetch_meta(stage + 1);
+            if (Loops == 1)
+                fetch_meta((stage + 1) * StageSteps);
         }
 #pragma clang loop unroll(disable)
         for (int u = 0; u < Loops; ++u) {       // (unrolled, smaller units would need more registers than there are)
+            // the next unit's scales are on their way while this one's are used
+            if (Loops > 1) {
+#pragma unroll
+                for (int j = 0; j < NC; ++j)
+                    mt[j] = mn[j];
+                if (u + 1 < Loops || stage + 1 < end)
+                    fetch_meta(stage * StageSteps + (u + 1) * LoopSteps);
+            }
             // a unit's sums start from what its offset takes off, - (16 + zero) times the sum of x
             if (StageSteps >= STEPS || !(stage & 1)) {
                 f32x4 xs[RT];
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
-                    xs[t] = *reinterpret_cast<const f32x4*>(&sums[half][u][t * 16 + kb * 4]);
+                    xs[t] = *reinterpret_cast<const f32x4*>(sums_now + u * Rows + t * 16 + kb * 4);
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
-                    uint32_t word = mt[j][0];
-#pragma unroll
-                    for (int k = 1; k < Loops; ++k)
-                        word = u == k ? mt[j][k] : word;
-                    const float offset = -(16.0f + (float)(word & 15u));
+                    const float offset = -(16.0f + (float)(mt[j] & 15u));
 #pragma unroll
                     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -311,7 +291,7 @@ q4_gemm_kernel(GemmArgs g)
                     u32x4 a[RT];
 #pragma unroll
                     for (int t = 0; t < RT; ++t)
-                        a[t] = *reinterpret_cast<const u32x4*>(tile[half] + (t * 16 + c) * RowBytes +
+                        a[t] = *reinterpret_cast<const u32x4*>(now + (t * 16 + c) * RowBytes +
                                                                place_of(c, (q * StageSteps + s) * 4 + kb) * 16);
 #pragma unroll
                     for (int j = 0; j < NC; ++j)
@@ -324,11 +304,7 @@ q4_gemm_kernel(GemmArgs g)
             if (StageSteps >= STEPS || (stage & 1)) {
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
-                    uint32_t word = mt[j][0];
-#pragma unroll
-                    for (int k = 1; k < Loops; ++k)
-                        word = u == k ? mt[j][k] : word;
-                    const float scale = __uint_as_float(word & ~15u);
+                    const float scale = __uint_as_float(mt[j] & ~15u);
 #pragma unroll
                     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -337,10 +313,30 @@ q4_gemm_kernel(GemmArgs g)
                 }
             }
         }
-        if (stage + 1 < end) {
-            put_x(half ^ 1);
+    };
+
+    if (first < end) {
+        fetch_x(first, tile[0]);
+        fetch_sums(first);
+        fetch_codes(first);
+        fetch_meta(first * StageSteps);
+        put_sums(0);
+    }
+    for (int stage = first, half = 0; stage < end; ++stage, half ^= 1) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int s = 0; s < StageSteps; ++s)
+                w[j][s] = wn[j][s];
+        if (Loops == 1)
+#pragma unroll
+            for (int j = 0; j < NC; ++j)
+                mt[j] = mn[j];
+        __builtin_amdgcn_s_waitcnt(0x0f70);     // vmcnt(0): this wave's part of the tile has landed
+        __syncthreads();        // this stage's tile is whole, and nobody reads the other any more
+        multiply(stage, tile[half], sums[half][0], tile[half ^ 1]);
+        if (stage + 1 < end)
             put_sums(half ^ 1);
-        }
     }
 
     // rows beyond M and columns beyond N lie outside the descriptors
