@@ -22,239 +22,308 @@ namespace nmspmm {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-__device__ inline int dense_row(int kept, int n, int m, int local) { return kept / n * m + local; }
-
-// One wave packs one block: lane 16 kb + c takes the 32 rows {32 s + 8 kb + e} of column c.
-// FROM_VALUES: the codes are found here, otherwise they are given.  HBM-bound: a wave instruction reads
-// four 64-byte row segments whose other half the neighbouring wave of the workgroup reads.
-template <bool FROM_VALUES>
-__global__ void __launch_bounds__(256)
-q4_pack_kernel(const float* __restrict__ values, const uint8_t* __restrict__ given, const float* __restrict__ scales,
-               const uint8_t* __restrict__ zeros, const int32_t* __restrict__ rows, Q4Shape p, bool asymmetric,
-               uint32_t* __restrict__ codes, uint32_t* __restrict__ meta)
-{
-    const int lane = threadIdx.x & 63, c = lane & 15, kb = lane >> 4;
-    const int tile = blockIdx.y * 4 + (threadIdx.x >> 6), block = blockIdx.x;
-    if (tile >= p.tiles)
-        return;
-    const int col = tile * 16 + c;
-    const bool column = col < p.N;
-    const int per = 128 / p.group;      // groups of a block: 1, 2 or 4
-    const int row0 = block * 128 + kb * 8;
-    uint32_t word[4];
-    uint32_t mt[4] = {0, 0, 0, 0};
-
-    if (FROM_VALUES) {
-        float v[4][8];
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int r = row0 + s * 32 + e;
-                v[s][e] = column && r < p.W ? __builtin_nontemporal_load(values + (size_t)r * p.N + col) : 0.0f;
-            }
-        // largest and smallest of each step over its 32 rows, zero among them; a NaN or an infinity
-        // anywhere makes the scale NaN (the whole group then expands to NaN)
-        float top[4], low[4];
-        bool bad[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            top[s] = low[s] = 0.0f;
-            bool odd = false;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                top[s] = fmaxf(top[s], v[s][e]);
-                low[s] = fminf(low[s], v[s][e]);
-                odd |= (__float_as_uint(v[s][e]) & 0x7f800000u) == 0x7f800000u;
-            }
-#pragma unroll
-            for (int mask = 16; mask < 64; mask <<= 1) {
-                top[s] = fmaxf(top[s], __shfl_xor(top[s], mask, 64));
-                low[s] = fminf(low[s], __shfl_xor(low[s], mask, 64));
-                odd |= __shfl_xor((int)odd, mask, 64) != 0;
-            }
-            bad[s] = odd;
-        }
-        if (per <= 2)
-#pragma unroll
-            for (int s = 0; s < 4; s += 2) {
-                top[s] = top[s + 1] = fmaxf(top[s], top[s + 1]);
-                low[s] = low[s + 1] = fminf(low[s], low[s + 1]);
-                bad[s] = bad[s + 1] = bad[s] || bad[s + 1];
-            }
-        if (per == 1) {
-            top[0] = top[1] = top[2] = top[3] = fmaxf(top[0], top[2]);
-            low[0] = low[1] = low[2] = low[3] = fminf(low[0], low[2]);
-            bad[0] = bad[1] = bad[2] = bad[3] = bad[0] || bad[2];
-        }
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            // the smallest scale of 20 significant bits with steps * scale >= what has to be covered
-            // (steps * scale has 24 bits at most: exact, and so is the comparison, in double)
-            const double steps = asymmetric ? 15.0 : 7.0;
-            const double need = asymmetric ? (double)top[s] - (double)low[s] : (double)fmaxf(top[s], -low[s]);
-            uint32_t bits = __float_as_uint((float)(need / steps)) & ~15u;
-            if (steps * (double)__uint_as_float(bits) < need)
-                bits += 16;
-            const float scale = __uint_as_float(bits);
-            float zero = 8.0f;
-            if (asymmetric)
-                zero = scale > 0.0f ? fminf(fmaxf((float)rint(-(double)low[s] / (double)scale), 0.0f), 15.0f) : 0.0f;
-            if (bad[s]) {
-                bits = 0x7fc00000u;
-                zero = 8.0f;
-            }
-            mt[s] = bits | (uint32_t)zero;
-            uint32_t w = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                // nearest whole number to value / scale, ties to even: the quotient of two floats can
-                // round onto a half that it only comes near, so the half is compared with the value
-                // itself (fma: one rounding, the sign of the difference is right)
-                float q = 0.0f;
-                if (scale > 0.0f && !bad[s]) {
-                    const float f = floorf(v[s][e] / scale);
-                    const float over = fmaf(-(f + 0.5f), scale, v[s][e]);
-                    q = over > 0.0f ? f + 1.0f : over < 0.0f ? f : 2.0f * rintf(0.5f * f + 0.25f);
-                }
-                q = row0 + s * 32 + e < p.W ? fminf(fmaxf(q + zero, 0.0f), 15.0f) : zero;
-                w |= (uint32_t)q << (4 * ((e >> 1) + 4 * (e & 1)));
-            }
-            word[s] = w;
-        }
-        const uint32_t all[4] = {mt[0], mt[1], mt[2], mt[3]};
-        if (per == 2)
-            mt[1] = all[2];
-    } else {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int j = block * per + g;
-            if (g < per && column && (size_t)j * p.group < (size_t)p.W) {
-                const uint32_t z = zeros ? zeros[(size_t)j * p.N + col] : 8u;
-                // 20 significant bits, to the nearest (ties away from zero; 16-bit scales are exact)
-                const uint32_t bits = __float_as_uint(scales[(size_t)j * p.N + col]);
-                const bool odd = (bits & 0x7f800000u) == 0x7f800000u;
-                mt[g] = ((odd ? 0x7fc00000u : bits + 8u) & ~15u) | (z & 15u);
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const uint32_t z = mt[s * per / 4] & 15u;
-            uint32_t w = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int r = row0 + s * 32 + e;
-                uint32_t q = z;      // rows beyond W count as zero
-                if (column && r < p.W) {
-                    q = given[(size_t)r * p.N + col] & 15u;
-                    if (rows) {     // a kept row outside its window counts as zero
-                        const int local = rows[(size_t)r * (p.N / 32) + (col >> 5)];
-                        if (local < 0 || local >= p.m)
-                            q = z;
-                    }
-                }
-                w |= q << (4 * ((e >> 1) + 4 * (e & 1)));
-            }
-            word[s] = w;
-        }
+// Nearest whole number to x / scale, ties to even, for |x| <= 16 scale and a scale of 20 significant bits.  The product with the
+// inverse gives it or its neighbour; what remains of x (exact: one fma, 23 bits at most) is compared with half a scale.
+// Tiny scales are made normal together with x, so that the inverse exists.
+struct Nearest {
+    float factor, scale, inverse, half, below;
+    __device__ explicit Nearest(float s)
+    {
+        factor = s < 0x1p-100f ? 0x1p100f : 1.0f;
+        scale = s * factor;
+        inverse = 1.0f / scale;
+        half = 0.5f * scale;
+        below = __uint_as_float(__float_as_uint(half) - 1);     // so that "more than it" is "half or more": an odd number does not keep a tie
     }
-    if (FROM_VALUES && rows) {
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int r = row0 + s * 32 + e;
-                if (column && r < p.W) {
-                    const int local = rows[(size_t)r * (p.N / 32) + (col >> 5)];
-                    const int at = 4 * ((e >> 1) + 4 * (e & 1));
-                    if (local < 0 || local >= p.m)
-                        word[s] = (word[s] & ~(15u << at)) | ((mt[s * per / 4] & 15u) << at);
-                }
-            }
+    __device__ float operator()(float x) const
+    {
+        x *= factor;
+        const float q = rintf(x * inverse), rest = fmaf(-q, scale, x);
+        const float most = ((int)q & 1) ? below : half;
+        return q + (rest > most ? 1.0f : rest < -most ? -1.0f : 0.0f);
     }
-    const size_t at = (size_t)tile * p.blocks + block;
-    *reinterpret_cast<u32x4*>(codes + (at * 64 + lane) * 4) = u32x4{word[0], word[1], word[2], word[3]};
-    if (kb == 0)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-            if (g < per)
-                meta[(at * 16 + c) * per + g] = mt[g];
-}
+};
 
-// rows[N/32][blocks*128]: one thread per entry, consecutive threads take consecutive vectors of a row
-// of DT (the reads coalesce; the bytes are written once in a model's life).
-__global__ void __launch_bounds__(256)
-q4_rows_kernel(const int32_t* __restrict__ rows, Q4Shape p, uint8_t* __restrict__ out)
+// Where row e of a word's eight lies: its nibble's first bit.
+__device__ constexpr int nibble(int e) { return 4 * ((e >> 1) + 4 * (e & 1)); }
+
+// The dense rows of a lane's eight kept rows, counted from the first row of their step; `keep` bit e: row e is inside its
+// window.  One that is not gets a row that its window does not keep (its code will be the zero point).
+__device__ inline void row_offsets(const int (&local)[8], int r0, const Q4Shape& p, int (&offset)[8], uint32_t& keep)
 {
-    const int Q = p.N / 32;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const int r = (int)(i / Q), v = (int)(i % Q);
-    if (r >= p.blocks * 128)
-        return;
-    int offset = 0;
-    if (r < p.W) {
-        int local = rows[i];
-        if (local < 0 || local >= p.m) {
-            // its code is the zero point: any row that the window does not keep will do
-            const int first = r / p.n * p.n;
-            for (local = 0; local < p.m; ++local) {
+    const int shift = __builtin_ctz(p.n);       // n is 1, 2, 4 or 8
+    keep = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        keep |= local[e] >= 0 && local[e] < p.m ? 1u << e : 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        int at = local[e];
+        if (!((keep >> e) & 1u)) {
+            for (at = 0; at < p.m; ++at) {
                 bool kept = false;
-                for (int k = 0; k < p.n; ++k)
-                    kept |= rows[(size_t)(first + k) * Q + v] == local;
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    kept |= k >> shift == e >> shift && local[k] == at;
                 if (!kept)
                     break;
             }
         }
-        offset = dense_row(r, p.n, p.m, local) - (r >> 5) * p.span;
+        offset[e] = ((r0 + e) >> shift) * p.m + at - (r0 >> 5) * p.span;
     }
-    out[(size_t)v * p.blocks * 128 + r] = (uint8_t)offset;
 }
 
-// Back to the dense fp32 matrix B[K][N].  One wave per block; a lane's eight rows of a step are whole
-// windows (n divides 8), so it writes all their dense rows: the kept ones and the zeros between.
-template <bool SPARSE>
+// A workgroup packs a block of 128 rows of 16 V columns, each of its four waves a step of 32 rows: lane 16 kb + c takes rows
+// 8 kb + e of columns V c .. V c + V - 1.  FROM_VALUES: the codes are found here, otherwise they are given.  HBM-bound, with
+// some 25 vector instructions a value to hide behind it: a wave holds a step and not a whole block (four columns and 128 rows
+// a wave: 4096 x 4096 34 us, two columns 28), a wave instruction reads four segments of 16 V values.
+template <bool FROM_VALUES, int V, bool SPARSE>
+__global__ void __launch_bounds__(256)
+q4_pack_kernel(const float* __restrict__ values, const uint8_t* __restrict__ given, const float* __restrict__ scales,
+               const uint8_t* __restrict__ zeros, const int32_t* __restrict__ rows, Q4Shape p, bool asymmetric,
+               uint32_t* __restrict__ codes, uint32_t* __restrict__ meta, uint8_t* __restrict__ offsets)
+{
+    constexpr int Cols = 16 * V;
+    __shared__ float tops[4][Cols], lows[4][Cols], odds[4][Cols];
+    __shared__ uint32_t groups[4][Cols];
+    __shared__ __attribute__((aligned(16))) uint32_t words[4 * Cols][4];    // [kb * Cols + column][step]
+    const int lane = threadIdx.x & 63, c = lane & 15, kb = lane >> 4, s = threadIdx.x >> 6;
+    const int block = blockIdx.y, first = blockIdx.x * Cols;    // neighbours run side by side: whole rows are in flight
+    const int col = first + c * V;      // the first of the lane's columns
+    const bool column = col < p.N;      // V divides N
+    const int per = 128 / p.group;      // groups of a block: 1, 2 or 4
+    const int g = per == 4 ? s : per == 2 ? s >> 1 : 0;     // this step's
+    const int r0 = block * 128 + s * 32 + kb * 8;
+
+    float v[8][V];
+    uint32_t x[8];      // given codes, a byte a column
+    if (FROM_VALUES) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            typedef float part __attribute__((ext_vector_type(V > 1 ? V : 2)));
+            const float* const at = values + (size_t)(r0 + e) * p.N + col;
+            const bool in = column && r0 + e < p.W;
+            if (V > 1) {
+                const part y = in ? __builtin_nontemporal_load(reinterpret_cast<const part*>(at)) : part(0.0f);
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    v[e][i] = y[i % (V > 1 ? V : 2)];
+            } else
+                v[e][0] = in ? __builtin_nontemporal_load(at) : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint8_t* const at = given + (size_t)(r0 + e) * p.N + col;
+            x[e] = 0;
+            if (column && r0 + e < p.W)
+                x[e] = V == 4 ? *reinterpret_cast<const uint32_t*>(at) : *at;
+        }
+    }
+    // which of the kept rows lie inside their windows, and the offsets of all
+    uint32_t keep = 255u;
+    if (SPARSE) {
+        const int Q = p.N / 32, vector = col >> 5;
+        int local[8], offset[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            local[e] = column && r0 + e < p.W ? rows[(size_t)(r0 + e) * Q + vector] : e & (p.n - 1);
+        row_offsets(local, r0, p, offset, keep);
+        if (column && (col & 31) == 0) {
+            uint2 eight = make_uint2(0, 0);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t byte = r0 + e < p.W ? (uint32_t)offset[e] & 255u : 0u;
+                if (e < 4)
+                    eight.x |= byte << (8 * (e & 3));
+                else
+                    eight.y |= byte << (8 * (e & 3));
+            }
+            *reinterpret_cast<uint2*>(offsets + (size_t)vector * p.blocks * 128 + r0) = eight;
+        }
+    }
+
+    uint32_t mt[V];
+    if (FROM_VALUES) {
+        // largest and smallest of each step, zero among them; a NaN or an infinity anywhere makes the scale NaN (the
+        // whole group then expands to NaN)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float top = 0.0f, low = 0.0f, odd = 0.0f;       // odd stays zero with finite numbers
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                top = fmaxf(top, v[e][i]);
+                low = fminf(low, v[e][i]);
+                odd = fmaf(v[e][i], 0.0f, odd);
+            }
+#pragma unroll
+            for (int mask = 16; mask < 64; mask <<= 1) {
+                top = fmaxf(top, __shfl_xor(top, mask, 64));
+                low = fminf(low, __shfl_xor(low, mask, 64));
+                odd += __shfl_xor(odd, mask, 64);
+            }
+            if (kb == 0) {
+                tops[s][c * V + i] = top;
+                lows[s][c * V + i] = low;
+                odds[s][c * V + i] = odd;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float top = 0.0f, low = 0.0f, odd = 0.0f;
+            for (int t = g * 4 / per; t < (g + 1) * 4 / per; ++t) {
+                top = fmaxf(top, tops[t][c * V + i]);
+                low = fminf(low, lows[t][c * V + i]);
+                odd += odds[t][c * V + i];
+            }
+            // The smallest scale of 20 significant bits with steps * scale >= what has to be covered: the quotient is near
+            // enough to be a step off at most (steps * scale has 24 bits: exact, and so is the comparison, in double).
+            const double steps = asymmetric ? 15.0 : 7.0;
+            const double need = asymmetric ? (double)top - (double)low : (double)fmaxf(top, -low);
+            uint32_t bits = __float_as_uint((float)need * (asymmetric ? 1.0f / 15.0f : 1.0f / 7.0f)) & ~15u;
+            if (steps * (double)__uint_as_float(bits) < need)
+                bits += 16;
+            else if (bits >= 16 && steps * (double)__uint_as_float(bits - 16) >= need)
+                bits -= 16;
+            const float scale = __uint_as_float(bits);
+            float zero = 8.0f;
+            if (asymmetric)
+                zero = scale > 0.0f ? fminf(fmaxf(Nearest(scale)(-low), 0.0f), 15.0f) : 0.0f;
+            mt[i] = odd != 0.0f ? 0x7fc00008u : bits | (uint32_t)zero;      // (odd is NaN)
+        }
+    } else {
+        const int j = block * per + g;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            mt[i] = 0;
+            if (column && (size_t)j * p.group < (size_t)p.W) {
+                const uint32_t z = zeros ? zeros[(size_t)j * p.N + col + i] : 8u;
+                // 20 significant bits, to the nearest (ties away from zero; 16-bit scales are exact)
+                const uint32_t bits = __float_as_uint(scales[(size_t)j * p.N + col + i]);
+                const bool odd = (bits & 0x7f800000u) == 0x7f800000u;
+                mt[i] = ((odd ? 0x7fc00000u : bits + 8u) & ~15u) | (z & 15u);
+            }
+        }
+    }
+    uint32_t in = 0;        // the nibbles of rows that count: not beyond W, not outside their window
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        in |= column && r0 + e < p.W && ((keep >> e) & 1u) ? 15u << nibble(e) : 0u;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float scale = __uint_as_float(mt[i] & ~15u), zero = (float)(mt[i] & 15u);
+        const Nearest nearest(scale);
+        uint32_t w = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (FROM_VALUES)
+                w |= (uint32_t)__builtin_amdgcn_fmed3f(nearest(v[e][i]) + zero, 0.0f, 15.0f) << nibble(e);
+            else
+                w |= ((x[e] >> (8 * i)) & 15u) << nibble(e);
+        }
+        const uint32_t mask = FROM_VALUES && !(scale > 0.0f) ? 0u : in;     // (nothing counts under a scale of 0 or NaN)
+        w = (w & mask) | ((mt[i] & 15u) * 0x11111111u & ~mask);
+        words[kb * Cols + c * V + i][s] = w;
+        if (kb == 0)
+            groups[g][c * V + i] = mt[i];
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < 4 * Cols; n += 256) {
+        const int part = n / Cols, at = first + n % Cols, tile = at >> 4;
+        if (tile < p.tiles)
+            *reinterpret_cast<u32x4*>(codes + (((size_t)tile * p.blocks + block) * 64 + part * 16 + (at & 15)) * 4) =
+                *reinterpret_cast<const u32x4*>(words[n]);
+    }
+    for (int n = threadIdx.x; n < per * Cols; n += 256) {
+        const int at = first + n / per, tile = at >> 4;
+        if (tile < p.tiles)
+            meta[(((size_t)tile * p.blocks + block) * 16 + (at & 15)) * per + n % per] = groups[n % per][n / per];
+    }
+}
+
+// Back to the dense fp32 matrix B[K][N], with the same split.  A lane's eight rows of a step are whole windows (KEPT = n divides
+// 8), so it writes all their dense rows: the kept ones and the zeros between.  KEPT 0: a dense operand.
+template <int KEPT, int V>
 __global__ void __launch_bounds__(256)
 q4_expand_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict__ meta, const uint8_t* __restrict__ rows,
                  Q4Shape p, float* __restrict__ B)
 {
     const int lane = threadIdx.x & 63, c = lane & 15, kb = lane >> 4;
-    const int tile = blockIdx.y * 4 + (threadIdx.x >> 6), block = blockIdx.x;
-    const int col = tile * 16 + c;
+    const int block = blockIdx.y;
+    const int col = (blockIdx.x * 4 + (threadIdx.x >> 6)) * (16 * V) + c * V;
     if (col >= p.N)
         return;
     const int per = 128 / p.group;
-    const size_t at = (size_t)tile * p.blocks + block;
-    const u32x4 word = *reinterpret_cast<const u32x4*>(codes + (at * 64 + lane) * 4);
+    const size_t at = (size_t)(col >> 4) * p.blocks + block;
+    const int place = col & 15;
+    u32x4 word[V];
+    uint32_t mt[V][4];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        word[i] = *reinterpret_cast<const u32x4*>(codes + (at * 64 + kb * 16 + place + i) * 4);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            if (g < per)
+                mt[i][g] = meta[(at * 16 + place + i) * per + g];
+    }
+    uint2 offs[4];
+    if (KEPT)
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            offs[s] = *reinterpret_cast<const uint2*>(rows + (size_t)(col >> 5) * p.blocks * 128 + block * 128 + s * 32 + kb * 8);
+    auto put = [&](int row, const float* x) {
+        float* const to = B + (size_t)row * p.N + col;
+        if (V == 4)
+            __builtin_nontemporal_store(f32x4{x[0], x[1 % V], x[2 % V], x[3 % V]}, reinterpret_cast<f32x4*>(to));
+        else
+            __builtin_nontemporal_store(x[0], to);
+    };
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        const uint32_t mt = meta[(at * 16 + c) * per + s * per / 4];
-        const float scale = __uint_as_float(mt & ~15u);
-        const int zero = (int)(mt & 15u);
-        float v[8];
+        float v[8][V];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            v[e] = scale * (float)((int)((word[s] >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) - zero);
+        for (int i = 0; i < V; ++i) {
+            const uint32_t m = per == 4 ? mt[i][s] : per == 2 ? mt[i][s >> 1] : mt[i][0];
+            const float scale = __uint_as_float(m & ~15u);
+            const int zero = (int)(m & 15u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e][i] = scale * (float)((int)((word[i][s] >> nibble(e)) & 15u) - zero);
+        }
         const int r0 = block * 128 + s * 32 + kb * 8;
-        if (!SPARSE) {
+        if (KEPT == 0) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (r0 + e < p.W)
-                    __builtin_nontemporal_store(v[e], B + (size_t)(r0 + e) * p.N + col);
+                    put(r0 + e, v[e]);
         } else {
-            const uint2 offs = *reinterpret_cast<const uint2*>(rows + (size_t)(col >> 5) * p.blocks * 128 + r0);
-            int at_row[8];
+            constexpr int n = KEPT ? KEPT : 1;
+            const int d0 = r0 / n * p.m;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)   // from the first dense row of the lane's windows
-                at_row[e] = r0 + e < p.W ? (int)(((e < 4 ? offs.x : offs.y) >> (8 * (e & 3))) & 255u) - kb * (p.span / 4) : -1;
-            const int d0 = r0 / p.n * p.m;
-            const int count = min(p.span / 4, p.K - d0);
-            for (int d = 0; d < count; ++d) {
-                float out = 0.0f;
+            for (int w = 0; w < 8 / n; ++w) {
+                if (r0 + w * n >= p.W)
+                    continue;
+                int place_of[n];        // of the window's kept rows
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    out = at_row[e] == d ? v[e] : out;
-                __builtin_nontemporal_store(out, B + (size_t)(d0 + d) * p.N + col);
+                for (int k = 0; k < n; ++k) {
+                    const int e = w * n + k;
+                    place_of[k] = (int)(((e < 4 ? offs[s].x : offs[s].y) >> (8 * (e & 3))) & 255u) - (kb * (8 / n) + w) * p.m;
+                }
+                for (int d = 0; d < p.m; ++d) {
+                    float out[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        out[i] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < n; ++k)
+#pragma unroll
+                        for (int i = 0; i < V; ++i)
+                            out[i] = place_of[k] == d ? v[w * n + k][i] : out[i];
+                    put(d0 + w * p.m + d, out);
+                }
             }
         }
     }
@@ -266,26 +335,46 @@ hipError_t launch_q4_pack(const float* values, const uint8_t* given, const float
                           const int32_t* rows, const Q4Shape& p, bool asymmetric, uint32_t* codes, uint32_t* meta,
                           uint8_t* row_offsets, hipStream_t stream)
 {
-    const dim3 grid(p.blocks, (p.tiles + 3) / 4);
-    if (values)
-        q4_pack_kernel<true><<<grid, 256, 0, stream>>>(values, nullptr, nullptr, nullptr, rows, p, asymmetric, codes, meta);
-    else
-        q4_pack_kernel<false><<<grid, 256, 0, stream>>>(nullptr, given, scales, zeros, rows, p, false, codes, meta);
-    if (rows) {
-        const size_t entries = (size_t)p.blocks * 128 * (p.N / 32);
-        q4_rows_kernel<<<(unsigned)((entries + 255) / 256), 256, 0, stream>>>(rows, p, row_offsets);
+    // four columns a lane where rows are whole pieces of four
+    const bool four = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(values) & 15u) == 0 && (reinterpret_cast<uintptr_t>(given) & 3u) == 0;
+    const dim3 grid(four ? (p.tiles + 3) / 4 : p.tiles, p.blocks);
+#define NMSPMM_PACK(FROM, V, SPARSE)                                                                                          \
+    q4_pack_kernel<FROM, V, SPARSE><<<grid, 256, 0, stream>>>(values, given, scales, zeros, rows, p, asymmetric, codes, meta, \
+                                                              row_offsets)
+    if (values) {
+        if (rows)
+            four ? NMSPMM_PACK(true, 4, true) : NMSPMM_PACK(true, 1, true);
+        else
+            four ? NMSPMM_PACK(true, 4, false) : NMSPMM_PACK(true, 1, false);
+    } else {
+        if (rows)
+            four ? NMSPMM_PACK(false, 4, true) : NMSPMM_PACK(false, 1, true);
+        else
+            four ? NMSPMM_PACK(false, 4, false) : NMSPMM_PACK(false, 1, false);
     }
+#undef NMSPMM_PACK
     return hipGetLastError();
 }
 
 hipError_t launch_q4_expand(const uint32_t* codes, const uint32_t* meta, const uint8_t* row_offsets, const Q4Shape& p,
                             float* B, hipStream_t stream)
 {
-    const dim3 grid(p.blocks, (p.tiles + 3) / 4);
-    if (row_offsets)
-        q4_expand_kernel<true><<<grid, 256, 0, stream>>>(codes, meta, row_offsets, p, B);
+    const bool four = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(B) & 15u) == 0;
+    const dim3 grid(four ? (p.tiles + 15) / 16 : (p.tiles + 3) / 4, p.blocks);
+#define NMSPMM_EXPAND(KEPT)                                                                                       \
+    (four ? q4_expand_kernel<KEPT, 4><<<grid, 256, 0, stream>>>(codes, meta, row_offsets, p, B)                   \
+          : q4_expand_kernel<KEPT, 1><<<grid, 256, 0, stream>>>(codes, meta, row_offsets, p, B))
+    if (!row_offsets)
+        NMSPMM_EXPAND(0);
+    else if (p.n == 1)
+        NMSPMM_EXPAND(1);
+    else if (p.n == 2)
+        NMSPMM_EXPAND(2);
+    else if (p.n == 4)
+        NMSPMM_EXPAND(4);
     else
-        q4_expand_kernel<false><<<grid, 256, 0, stream>>>(codes, meta, row_offsets, p, B);
+        NMSPMM_EXPAND(8);
+#undef NMSPMM_EXPAND
     return hipGetLastError();
 }
 

@@ -136,14 +136,24 @@ class NMSparseLinear(torch.nn.Module):
 _TYPES = {torch.float32: _nm.F32, torch.bfloat16: _nm.BF16, torch.float16: _nm.F16}
 
 
-def _on(device):
-    """The stream that calls for tensors on this device go to (its current one), as an integer."""
-    return torch.cuda.current_stream(device).cuda_stream
+# the current stream of a device, by its index, as an integer (without a Stream object, which takes longer than a launch)
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _guard(tensor):
-    """Makes the tensor's device the current one (kernels are launched there) where it is not."""
+    """Makes the tensor's device the current one (kernels are launched there)."""
     return torch.cuda.device(tensor.device)
+
+
+def _on_device(call, index, *args):
+    """call(*args, the device's current stream), with that device as the current one; raises what the status says."""
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            status = call(*args, _stream_of(index))
+    else:
+        status = call(*args, _stream_of(index))
+    if status != _nm.OK:
+        raise _nm.NmSpmmError(call.__name__, status)
 
 
 class NMQuantOperand:
@@ -222,28 +232,20 @@ def _quant_linear(x, operand):
     M = y.numel() // N
     if M == 0:
         return y
-    if x.dim() != 2:
+    ldx = K
+    if not x.is_contiguous():
         x = x.reshape(M, K)
-    ldx = x.stride(0) if M > 1 else K
-    if (K > 1 and x.stride(1) != 1) or ldx < K:
-        x, ldx = x.contiguous(), K
-    device = x.device
-    if device.index != torch.cuda.current_device():
-        with _guard(x):
-            return _launch_quant_linear(x, ldx, y, N, M, operand, device)
-    return _launch_quant_linear(x, ldx, y, N, M, operand, device)
-
-
-def _launch_quant_linear(x, ldx, y, ldy, M, operand, device):
+        ldx = x.stride(0) if M > 1 else K
+        if (K > 1 and x.stride(1) != 1) or ldx < K or ldx > 1 << 24:
+            x, ldx = x.contiguous(), K
     type_, need, space = _TYPES[x.dtype], 0, None
+    lib = _nm.lib()
     if M > 8:       # below, no operand needs a workspace
-        need = _nm.lib().nmspmm_q4_workspace_bytes(M, operand.K, operand.N, operand.n, operand.m, type_)
+        need = lib.nmspmm_q4_workspace_bytes(M, K, N, operand.n, operand.m, type_)
         if need:
             workspace = x.new_empty(need, dtype=torch.uint8)    # from torch's caching allocator, ordered on the stream
             space = workspace.data_ptr()
-    status = _nm.lib().nmspmm_q4_linear(operand, x.data_ptr(), ldx, y.data_ptr(), ldy, M, type_, space, need, _on(device))
-    if status != _nm.OK:
-        raise _nm.NmSpmmError("nmspmm_q4_linear", status)
+    _on_device(lib.nmspmm_q4_linear, x.get_device(), operand, x.data_ptr(), ldx, y.data_ptr(), N, M, type_, space, need)
     return y
 
 
@@ -389,14 +391,7 @@ def _block_norm_forward(residual, branch, params, factor, post, pre, eps, weight
     if residual.numel() == 0:
         return total, out, stats
     packed, keep = _pack_block_norm(residual, branch, total, out, stats, params, factor, post, pre, eps, weight_offset, gate_rows, dtype)
-    device = residual.device
-    if device.index != torch.cuda.current_device():
-        with _guard(residual):
-            status = _nm.lib().nmspmm_block_norm_forward(packed, _on(device))
-    else:
-        status = _nm.lib().nmspmm_block_norm_forward(packed, _on(device))
-    if status != _nm.OK:
-        raise _nm.NmSpmmError("nmspmm_block_norm_forward", status)
+    _on_device(_nm.lib().nmspmm_block_norm_forward, residual.get_device(), packed)
     return total, out, stats
 
 
@@ -417,13 +412,10 @@ def _block_norm_backward(residual, branch, params, stats, grad_sum, grad_out, fa
     total, out = (None if branch is None else residual), (stats if want_out else None)
     packed, keep = _pack_block_norm(residual, branch, total, out, stats, params, factor, post, pre, eps, weight_offset, gate_rows, dtype)
     want = _nm.BLOCK_NORM_GRADS.pack(ld_sum, ld_out, D, D, _at(grad_sum), _at(grad_out), *[_at(g) for g in grads])
-    with _guard(residual):
-        rows = residual.numel() // D
-        bytes_ = _nm.lib().nmspmm_block_norm_workspace_bytes(rows, gate_rows, D)
-        workspace = residual.new_empty(bytes_ // 4, dtype=torch.float32)
-        status = _nm.lib().nmspmm_block_norm_backward(packed, want, workspace.data_ptr(), bytes_, _on(residual.device))
-    if status != _nm.OK:
-        raise _nm.NmSpmmError("nmspmm_block_norm_backward", status)
+    lib = _nm.lib()
+    need = lib.nmspmm_block_norm_workspace_bytes(residual.numel() // D, gate_rows, D)
+    workspace = residual.new_empty(need // 4, dtype=torch.float32)
+    _on_device(lib.nmspmm_block_norm_backward, residual.get_device(), packed, want, workspace.data_ptr(), need)
     return grads
 
 
