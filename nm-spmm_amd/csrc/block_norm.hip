@@ -125,30 +125,66 @@ __device__ inline void store8(void* p, int type, size_t row, int t, int stride, 
     }
 }
 
+// The sum over a wave, in every lane: neighbours, quads and rows of 16 by lane permutation within the vector unit, rows and halves by
+// swapping them (an exchange through LDS takes ten times as long, and a row waits for six of them in turn).
+template <int CTRL>
+__device__ inline float exchanged(float v)
+{
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+__device__ inline float wave_sum(float v)
+{
+    v += exchanged<0xb1>(v);        // lane ^ 1
+    v += exchanged<0x4e>(v);        // lane ^ 2
+    v += exchanged<0x141>(v);       // the other quad of eight
+    v += exchanged<0x140>(v);       // the other half of sixteen
+    const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(rows[0]) + __uint_as_float(rows[1]);
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+}
+
 // Sums over the threads of a row: a wave, or the workgroup's waves through LDS (two halves used in turn: one barrier a sum).
 struct RowSum {
     float (*slots)[2][kMaxThreads / 64];
     int half, waves;
-    __device__ void operator()(float& a, float& b)
+    template <bool BOTH>
+    __device__ void add(float& a, float& b)
     {
-#pragma unroll
-        for (int mask = 1; mask < 64; mask <<= 1) {
-            a += __shfl_xor(a, mask, 64);
-            b += __shfl_xor(b, mask, 64);
-        }
+        a = wave_sum(a);
+        if (BOTH)
+            b = wave_sum(b);
         if (waves == 1)
             return;
         if ((threadIdx.x & 63) == 0) {
             slots[half][0][threadIdx.x >> 6] = a;
-            slots[half][1][threadIdx.x >> 6] = b;
+            if (BOTH)
+                slots[half][1][threadIdx.x >> 6] = b;
         }
         __syncthreads();
-        a = b = 0.0f;
-        for (int w = 0; w < waves; ++w) {
-            a += slots[half][0][w];
-            b += slots[half][1][w];
+        // (slots of waves that there are not hold zero)
+        const float4* const from = reinterpret_cast<const float4*>(slots[half][0]);
+        const float4 p = from[0], q = from[1], r = from[2], s = from[3];
+        a = (((p.x + p.y) + (p.z + p.w)) + ((q.x + q.y) + (q.z + q.w))) + (((r.x + r.y) + (r.z + r.w)) + ((s.x + s.y) + (s.z + s.w)));
+        if (BOTH) {
+            const float4* const other = reinterpret_cast<const float4*>(slots[half][1]);
+            const float4 t = other[0], u = other[1], v = other[2], w = other[3];
+            b = (((t.x + t.y) + (t.z + t.w)) + ((u.x + u.y) + (u.z + u.w))) + (((v.x + v.y) + (v.z + v.w)) + ((w.x + w.y) + (w.z + w.w)));
         }
         half ^= 1;
+    }
+    __device__ void operator()(float& a)
+    {
+        float none = 0.0f;
+        add<false>(a, none);
+    }
+    __device__ void operator()(float& a, float& b) { add<true>(a, b); }
+
+    static __device__ void clear(float (*slots)[2][kMaxThreads / 64])
+    {
+        if (threadIdx.x < 4 * (kMaxThreads / 64))
+            slots[0][0][threadIdx.x] = 0.0f;
+        __syncthreads();
     }
 };
 
@@ -156,23 +192,23 @@ struct RowSum {
 template <int E>
 __device__ inline void standardize(float* v, const bool* in, int kind, float inv_d, float eps, RowSum& sum, float& mean, float& inv)
 {
-    float a = 0.0f, b = 0.0f;
+    float a = 0.0f;
     mean = 0.0f;
     if (kind == kLayerNorm) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
             a += v[e];
-        sum(a, b);
+        sum(a);
         mean = a * inv_d;
 #pragma unroll
         for (int e = 0; e < E; ++e)
             v[e] = in[e] ? v[e] - mean : 0.0f;
-        a = b = 0.0f;
+        a = 0.0f;
     }
 #pragma unroll
     for (int e = 0; e < E; ++e)
         a = fmaf(v[e], v[e], a);
-    sum(a, b);
+    sum(a);
     inv = 1.0f / sqrtf(a * inv_d + eps);
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -180,9 +216,10 @@ __device__ inline void standardize(float* v, const bool* in, int kind, float inv
 }
 
 // The thread's columns of the parameters (1, 0 or the plain factor where there is none).
-template <bool VEC, int NV>
+template <bool VEC, int NV, bool BIAS>
 struct Columns {
-    float post_w[NV * 8], post_b[NV * 8], scale[NV * 8], pre_w[NV * 8], pre_b[NV * 8], gate[NV * 8];
+    float post_w[NV * 8], scale[NV * 8], pre_w[NV * 8], gate[NV * 8];
+    float post_b[BIAS ? NV * 8 : 8], pre_b[BIAS ? NV * 8 : 8];
 
     // everything that does not change from row to row: all loads first, then their values
     __device__ void load(const BlockNormArgs& a, size_t gate_row, bool with_gate, int t, int stride)
@@ -192,13 +229,13 @@ struct Columns {
         for (int v = 0; v < NV; ++v) {
             if (a.post_weight.data)
                 pw[v] = load_raw<VEC>(a.post_weight.data, a.post_weight.type, 0, t, stride, v, a.D);
-            if (a.post_bias.data)
+            if (BIAS && a.post_bias.data)
                 pb[v] = load_raw<VEC>(a.post_bias.data, a.post_bias.type, 0, t, stride, v, a.D);
             if (a.scale.data)
                 sc[v] = load_raw<VEC>(a.scale.data, a.scale.type, 0, t, stride, v, a.D);
             if (a.pre_weight.data)
                 nw[v] = load_raw<VEC>(a.pre_weight.data, a.pre_weight.type, 0, t, stride, v, a.D);
-            if (a.pre_bias.data)
+            if (BIAS && a.pre_bias.data)
                 nb[v] = load_raw<VEC>(a.pre_bias.data, a.pre_bias.type, 0, t, stride, v, a.D);
             if (with_gate)
                 g[v] = load_raw<VEC>(a.gate.data, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D);
@@ -206,10 +243,12 @@ struct Columns {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             value(a.post_weight, pw[v], 1.0f, a.weight_offset, post_w + v * 8);
-            value(a.post_bias, pb[v], 0.0f, 0.0f, post_b + v * 8);
+            if (BIAS)
+                value(a.post_bias, pb[v], 0.0f, 0.0f, post_b + v * 8);
             value(a.scale, sc[v], a.factor, 0.0f, scale + v * 8);
             value(a.pre_weight, nw[v], 1.0f, a.weight_offset, pre_w + v * 8);
-            value(a.pre_bias, nb[v], 0.0f, 0.0f, pre_b + v * 8);
+            if (BIAS)
+                value(a.pre_bias, nb[v], 0.0f, 0.0f, pre_b + v * 8);
             if (with_gate)
                 unpack<VEC>(g[v], a.gate.type, gate + v * 8);
             else
@@ -242,11 +281,12 @@ private:
 
 // ---- forward ------------------------------------------------------------------------------------------
 
-template <ElementType T, ElementType R, bool VEC, int NV>
+template <ElementType T, ElementType R, bool VEC, int NV, bool BIAS>
 __global__ void __launch_bounds__(kMaxThreads)
 block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
 {
-    __shared__ float slots[2][2][kMaxThreads / 64];
+    __shared__ __attribute__((aligned(16))) float slots[2][2][kMaxThreads / 64];
+    RowSum::clear(slots);
     constexpr int E = NV * 8;
     const int t = threadIdx.x % row_threads;
     const int walker = blockIdx.x * (blockDim.x / row_threads) + threadIdx.x / row_threads;
@@ -273,7 +313,7 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
     };
     if (begin < end)
         load(begin);
-    Columns<VEC, NV> p;
+    Columns<VEC, NV, BIAS> p;
     size_t gate_row = begin / a.gate_rows;
     p.load(a, gate_row, gated, t, stride);
 
@@ -300,7 +340,7 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
                 post_inv = inv;
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    y[e] = fmaf(y[e], p.post_w[e], p.post_b[e]);
+                    y[e] = BIAS ? fmaf(y[e], p.post_w[e], p.post_b[e]) : y[e] * p.post_w[e];
             }
 #pragma unroll
             for (int e = 0; e < E; ++e)
@@ -321,7 +361,7 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
                 pre_inv = inv;
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    s[e] = fmaf(s[e], p.pre_w[e], p.pre_b[e]);
+                    s[e] = BIAS ? fmaf(s[e], p.pre_w[e], p.pre_b[e]) : s[e] * p.pre_w[e];
             }
 #pragma unroll
             for (int v = 0; v < NV; ++v)
@@ -334,11 +374,12 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
 
 // ---- backward -----------------------------------------------------------------------------------------
 
-template <ElementType T, ElementType R, bool VEC, int NV, int THREADS>
+template <ElementType T, ElementType R, bool VEC, int NV, int THREADS, bool BIAS>
 __global__ void __launch_bounds__(THREADS)
 block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, int walkers, int per_gate, int gates_each)
 {
-    __shared__ float slots[2][2][kMaxThreads / 64];
+    __shared__ __attribute__((aligned(16))) float slots[2][2][kMaxThreads / 64];
+    RowSum::clear(slots);
     constexpr int E = NV * 8;
     const int t = threadIdx.x % row_threads;
     const int walker = blockIdx.x * (blockDim.x / row_threads) + threadIdx.x / row_threads;
@@ -360,17 +401,25 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
     RowSum sum = {slots, 0, row_threads / 64};
     const bool branch = a.branch != nullptr, gated = branch && a.gate.data != nullptr;
 
-    Columns<VEC, NV> p;
+    Columns<VEC, NV, BIAS> p;
     size_t gate_row = begin / a.gate_rows;
     p.load(a, gate_row, gated, t, stride);
-    float sum_post_w[E], sum_post_b[E], sum_scale[E], sum_pre_w[E], sum_pre_b[E], sum_gate[E];
+    float sum_post_w[E], sum_scale[E], sum_pre_w[E], sum_gate[E], sum_post_b[BIAS ? E : 8], sum_pre_b[BIAS ? E : 8];
 #pragma unroll
     for (int e = 0; e < E; ++e)
-        sum_post_w[e] = sum_post_b[e] = sum_scale[e] = sum_pre_w[e] = sum_pre_b[e] = sum_gate[e] = 0.0f;
+    {
+        sum_post_w[e] = sum_scale[e] = sum_pre_w[e] = sum_gate[e] = 0.0f;
+        if (BIAS)
+            sum_post_b[e] = sum_pre_b[e] = 0.0f;
+    }
 
-    for (size_t row = begin; row < end; ++row) {
-        Raw rr[NV], yr[NV], gs[NV], go[NV];
-        const float4 st = *reinterpret_cast<const float4*>(a.stats + row * 4);
+    auto after = [&](float y, int e) { return BIAS ? fmaf(y, p.post_w[e], p.post_b[e]) : y * p.post_w[e]; };
+
+    // the next row is on its way while one is worked on
+    Raw rr[NV], yr[NV], gs[NV], go[NV];
+    float4 stats = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto load = [&](size_t row) {
+        stats = *reinterpret_cast<const float4*>(a.stats + row * 4);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             rr[v] = load_raw<VEC>(a.residual, R, row * a.ld_residual, t, stride, v, a.D);
@@ -381,6 +430,11 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
             if (d.out)
                 go[v] = load_raw<VEC>(d.out, T, row * d.ld_out, t, stride, v, a.D);
         }
+    };
+    if (begin < end)
+        load(begin);
+    for (size_t row = begin; row < end; ++row) {
+        const float4 st = stats;
         if (gated && row / a.gate_rows != gate_row) {
             if (d.gate && per_gate == 1)
 #pragma unroll
@@ -392,7 +446,7 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
             gate_row = row / a.gate_rows;
             p.load_gate(a, gate_row, t, stride);
         }
-        float r[E], yn[E], s[E], ds[E];
+        float r[E], yn[E], s[E], ds[E], g[E];
 #pragma unroll
         for (int v = 0; v < NV; ++v)
             unpack<VEC>(rr[v], R, r + v * 8);
@@ -403,7 +457,7 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 yn[e] = (yn[e] - st.x) * st.y;      // mean 0 and 1 / deviation 1 where there is no norm
-                s[e] = fmaf(r[e], p.scale[e], fmaf(yn[e], p.post_w[e], p.post_b[e]) * p.gate[e]);
+                s[e] = fmaf(r[e], p.scale[e], after(yn[e], e) * p.gate[e]);
             }
         } else
 #pragma unroll
@@ -417,17 +471,20 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 ds[e] = 0.0f;
-        if (d.out) {
-            float g[E];
+        if (d.out)
 #pragma unroll
             for (int v = 0; v < NV; ++v)
                 unpack<VEC>(go[v], T, g + v * 8);   // zeros beyond D
+        if (row + 1 < end)
+            load(row + 1);
+        if (d.out) {
             float with = 0.0f, plain = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 s[e] = (s[e] - st.z) * st.w;
                 sum_pre_w[e] = fmaf(g[e], s[e], sum_pre_w[e]);
-                sum_pre_b[e] += g[e];
+                if (BIAS)
+                    sum_pre_b[e] += g[e];
                 g[e] *= p.pre_w[e];
                 with = fmaf(g[e], s[e], with);
                 plain += g[e];
@@ -455,11 +512,12 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
             if (column_of<VEC>(t, stride, e / 8, e % 8) >= a.D)
                 ds[e] = 0.0f;
             sum_scale[e] = fmaf(ds[e], r[e], sum_scale[e]);
-            sum_gate[e] = fmaf(ds[e], fmaf(yn[e], p.post_w[e], p.post_b[e]), sum_gate[e]);
+            sum_gate[e] = fmaf(ds[e], after(yn[e], e), sum_gate[e]);
             r[e] = ds[e] * p.scale[e];
             ds[e] *= p.gate[e];
             sum_post_w[e] = fmaf(ds[e], yn[e], sum_post_w[e]);
-            sum_post_b[e] += ds[e];
+            if (BIAS)
+                sum_post_b[e] += ds[e];
             ds[e] *= p.post_w[e];
             with = fmaf(ds[e], yn[e], with);
             plain += ds[e];
@@ -495,10 +553,12 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
                 store8<VEC>(d.partial, kF32, ((size_t)slot * walkers + walker) * a.D, t, stride, v, a.D, x + v * 8);
     };
     leave(d.slot_post_weight, sum_post_w);
-    leave(d.slot_post_bias, sum_post_b);
+    if (BIAS)
+        leave(d.slot_post_bias, sum_post_b);
     leave(d.slot_scale, sum_scale);
     leave(d.slot_pre_weight, sum_pre_w);
-    leave(d.slot_pre_bias, sum_pre_b);
+    if (BIAS)
+        leave(d.slot_pre_bias, sum_pre_b);
     leave(d.slot_gate, sum_gate);
 }
 
@@ -576,10 +636,12 @@ void forward(const BlockNormArgs& a, hipStream_t stream)
     const size_t most = (size_t)machine().cus * 16 / (rt / 64);
     const int walkers = (int)(a.rows < most ? a.rows : most);
     const dim3 grid((walkers + each - 1) / each), block(rt * each);
+    const bool bias = a.post_bias.data || a.pre_bias.data;
     if (a.D <= 8 * kMaxThreads)
-        block_norm_kernel<T, R, VEC, 1><<<grid, block, 0, stream>>>(a, rt, walkers);
+        bias ? block_norm_kernel<T, R, VEC, 1, true><<<grid, block, 0, stream>>>(a, rt, walkers)
+             : block_norm_kernel<T, R, VEC, 1, false><<<grid, block, 0, stream>>>(a, rt, walkers);
     else
-        block_norm_kernel<T, R, VEC, 2><<<grid, block, 0, stream>>>(a, rt, walkers);
+        block_norm_kernel<T, R, VEC, 2, true><<<grid, block, 0, stream>>>(a, rt, walkers);
 }
 
 template <ElementType T, ElementType R, bool VEC>
@@ -587,12 +649,16 @@ void backward(const BlockNormArgs& a, const BlockNormGrads& d, const BlockNormWa
 {
     const int rt = row_threads_of(a.D), each = rt == 64 ? 4 : 1;
     const dim3 grid((w.walkers + each - 1) / each), block(rt * each);
+    const bool bias = a.post_bias.data || a.pre_bias.data;
+#define NMSPMM_BACKWARD(NV, THREADS, BIAS) \
+    block_norm_backward_kernel<T, R, VEC, NV, THREADS, BIAS><<<grid, block, 0, stream>>>(a, d, rt, w.walkers, w.per_gate, w.gates_each)
     if (a.D <= 4096)
-        block_norm_backward_kernel<T, R, VEC, 1, 512><<<grid, block, 0, stream>>>(a, d, rt, w.walkers, w.per_gate, w.gates_each);
+        bias ? NMSPMM_BACKWARD(1, 512, true) : NMSPMM_BACKWARD(1, 512, false);
     else if (a.D <= 8 * kMaxThreads)
-        block_norm_backward_kernel<T, R, VEC, 1, 1024><<<grid, block, 0, stream>>>(a, d, rt, w.walkers, w.per_gate, w.gates_each);
+        bias ? NMSPMM_BACKWARD(1, 1024, true) : NMSPMM_BACKWARD(1, 1024, false);
     else
-        block_norm_backward_kernel<T, R, VEC, 2, 1024><<<grid, block, 0, stream>>>(a, d, rt, w.walkers, w.per_gate, w.gates_each);
+        NMSPMM_BACKWARD(2, 1024, true);
+#undef NMSPMM_BACKWARD
 }
 
 } // namespace
