@@ -35,93 +35,82 @@ __device__ inline uint32_t to_bits16(float v, int type)
     return __builtin_bit_cast(uint16_t, (_Float16)v);
 }
 
-// The columns of a thread: VEC: 8 consecutive ones, `stride` threads times 8 between its groups of eight; otherwise single
-// ones, `stride` apart.
-template <bool VEC>
-__device__ inline int column_of(int t, int stride, int v, int e)
+// The columns of a thread: eight consecutive ones, `stride` threads times eight between its groups of eight.  Where those reach
+// beyond a row's end, the row's last eight (WIDE: rows of eight and more); what of them another thread has, or no one, does
+// not count (owns).  So every access is 16 or 32 bytes, without a branch, and rows need no alignment beyond their elements'.
+template <bool WIDE>
+__device__ inline int column_of(int t, int stride, int v, int D)
 {
-    return VEC ? (t + v * stride) * 8 + e : t + (v * 8 + e) * stride;
+    const int c = (t + v * stride) * 8;
+    return WIDE ? min(c, D - 8) : c;
+}
+template <bool WIDE>
+__device__ inline bool owns(int t, int stride, int v, int e, int D)
+{
+    const int c = column_of<WIDE>(t, stride, v, D) + e;
+    return c >= (t + v * stride) * 8 && c < D;
 }
 
 // Eight elements as they lie in memory: loads of several tensors can be under way before the first is unpacked.
 struct Raw {
     u32x4 a, b;
 };
-template <bool VEC>
+template <bool WIDE>
 __device__ inline Raw load_raw(const void* p, int type, size_t row, int t, int stride, int v, int D)
 {
-    Raw r = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
-    if (VEC) {
-        const int c = column_of<true>(t, stride, v, 0);
-        if (c < D) {
-            if (type == kF32) {
-                const u32x4* const q = reinterpret_cast<const u32x4*>(static_cast<const float*>(p) + row + c);
-                r.a = q[0];
-                r.b = q[1];
-            } else
-                r.a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + row + c);
-        }
-    } else {
+    Raw r;
+    const int c = column_of<WIDE>(t, stride, v, D);
+    if (type == kF32) {
+        const float* const q = static_cast<const float*>(p) + row;
+        if (WIDE)
+            __builtin_memcpy(&r, q + c, 32);
+        else
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = column_of<false>(t, stride, v, e);
-            uint32_t x = 0;
-            if (c < D)
-                x = type == kF32 ? static_cast<const uint32_t*>(p)[row + c] : static_cast<const uint16_t*>(p)[row + c];
-            if (e < 4)
-                r.a[e] = x;
-            else
-                r.b[e - 4] = x;
-        }
+            for (int e = 0; e < 8; ++e)
+                (e < 4 ? r.a : r.b)[e & 3] = __float_as_uint(q[min(c + e, D - 1)]);
+    } else {
+        const uint16_t* const q = static_cast<const uint16_t*>(p) + row;
+        if (WIDE)
+            __builtin_memcpy(&r.a, q + c, 16);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                r.a[e] = q[min(c + 2 * e, D - 1)] | (uint32_t)q[min(c + 2 * e + 1, D - 1)] << 16;
     }
     return r;
 }
-template <bool VEC>
 __device__ inline void unpack(const Raw& r, int type, float* out)
 {
-    if (type == kF32) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            out[e] = __uint_as_float(e < 4 ? r.a[e & 3] : r.b[e & 3]);
-    } else if (VEC) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            out[e] = from_bits16(e & 1 ? r.a[e >> 1] >> 16 : r.a[e >> 1] & 0xffffu, type);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            out[e] = from_bits16(e < 4 ? r.a[e & 3] : r.b[e & 3], type);
-    }
+    for (int e = 0; e < 8; ++e)
+        out[e] = type == kF32 ? __uint_as_float(e < 4 ? r.a[e & 3] : r.b[e & 3])
+                              : from_bits16(e & 1 ? r.a[e >> 1] >> 16 : r.a[e >> 1] & 0xffffu, type);
 }
-template <bool VEC>
+template <bool WIDE>
 __device__ inline void store8(void* p, int type, size_t row, int t, int stride, int v, int D, const float* x)
 {
-    if (VEC) {
-        const int c = column_of<true>(t, stride, v, 0);
-        if (c >= D)
-            return;
-        if (type == kF32) {
-            u32x4* const q = reinterpret_cast<u32x4*>(static_cast<float*>(p) + row + c);
-            q[0] = u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
-            q[1] = u32x4{__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])};
-        } else {
-            u32x4 w;
+    const int c = (t + v * stride) * 8;
+    const bool whole = c + 8 <= D;
+    u32x4 w;
+    if (type != kF32)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                w[e] = to_bits16(x[2 * e], type) | to_bits16(x[2 * e + 1], type) << 16;
-            *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + row + c) = w;
-        }
-    } else {
+        for (int e = 0; e < 4; ++e)
+            w[e] = to_bits16(x[2 * e], type) | to_bits16(x[2 * e + 1], type) << 16;
+    if (whole) {
+        if (type == kF32)
+            __builtin_memcpy(static_cast<float*>(p) + row + c, x, 32);
+        else
+            __builtin_memcpy(static_cast<uint16_t*>(p) + row + c, &w, 16);
+    } else if (c < D) {
+        const int first = column_of<WIDE>(t, stride, v, D);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int c = column_of<false>(t, stride, v, e);
-            if (c >= D)
-                continue;
-            if (type == kF32)
-                static_cast<float*>(p)[row + c] = x[e];
-            else
-                static_cast<uint16_t*>(p)[row + c] = (uint16_t)to_bits16(x[e], type);
-        }
+        for (int e = 0; e < 8; ++e)
+            if (owns<WIDE>(t, stride, v, e, D)) {
+                if (type == kF32)
+                    static_cast<float*>(p)[row + first + e] = x[e];
+                else
+                    static_cast<uint16_t*>(p)[row + first + e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            }
     }
 }
 
@@ -216,7 +205,7 @@ __device__ inline void standardize(float* v, const bool* in, int kind, float inv
 }
 
 // The thread's columns of the parameters (1, 0 or the plain factor where there is none).
-template <bool VEC, int NV, bool BIAS>
+template <bool WIDE, int NV, bool BIAS>
 struct Columns {
     float post_w[NV * 8], scale[NV * 8], pre_w[NV * 8], gate[NV * 8];
     float post_b[BIAS ? NV * 8 : 8], pre_b[BIAS ? NV * 8 : 8];
@@ -228,17 +217,17 @@ struct Columns {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             if (a.post_weight.data)
-                pw[v] = load_raw<VEC>(a.post_weight.data, a.post_weight.type, 0, t, stride, v, a.D);
+                pw[v] = load_raw<WIDE>(a.post_weight.data, a.post_weight.type, 0, t, stride, v, a.D);
             if (BIAS && a.post_bias.data)
-                pb[v] = load_raw<VEC>(a.post_bias.data, a.post_bias.type, 0, t, stride, v, a.D);
+                pb[v] = load_raw<WIDE>(a.post_bias.data, a.post_bias.type, 0, t, stride, v, a.D);
             if (a.scale.data)
-                sc[v] = load_raw<VEC>(a.scale.data, a.scale.type, 0, t, stride, v, a.D);
+                sc[v] = load_raw<WIDE>(a.scale.data, a.scale.type, 0, t, stride, v, a.D);
             if (a.pre_weight.data)
-                nw[v] = load_raw<VEC>(a.pre_weight.data, a.pre_weight.type, 0, t, stride, v, a.D);
+                nw[v] = load_raw<WIDE>(a.pre_weight.data, a.pre_weight.type, 0, t, stride, v, a.D);
             if (BIAS && a.pre_bias.data)
-                nb[v] = load_raw<VEC>(a.pre_bias.data, a.pre_bias.type, 0, t, stride, v, a.D);
+                nb[v] = load_raw<WIDE>(a.pre_bias.data, a.pre_bias.type, 0, t, stride, v, a.D);
             if (with_gate)
-                g[v] = load_raw<VEC>(a.gate.data, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D);
+                g[v] = load_raw<WIDE>(a.gate.data, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D);
         }
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -250,7 +239,7 @@ struct Columns {
             if (BIAS)
                 value(a.pre_bias, nb[v], 0.0f, 0.0f, pre_b + v * 8);
             if (with_gate)
-                unpack<VEC>(g[v], a.gate.type, gate + v * 8);
+                unpack(g[v], a.gate.type, gate + v * 8);
             else
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -261,14 +250,14 @@ struct Columns {
     {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
-            unpack<VEC>(load_raw<VEC>(a.gate.data, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D), a.gate.type, gate + v * 8);
+            unpack(load_raw<WIDE>(a.gate.data, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D), a.gate.type, gate + v * 8);
     }
 
 private:
     __device__ static void value(const BlockNormVec& p, const Raw& r, float missing, float offset, float* out)
     {
         if (p.data) {
-            unpack<VEC>(r, p.type, out);
+            unpack(r, p.type, out);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 out[e] += offset;
@@ -281,7 +270,7 @@ private:
 
 // ---- forward ------------------------------------------------------------------------------------------
 
-template <ElementType T, ElementType R, bool VEC, int NV, bool BIAS>
+template <ElementType T, ElementType R, bool WIDE, int NV, bool BIAS>
 __global__ void __launch_bounds__(kMaxThreads)
 block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
 {
@@ -299,42 +288,52 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
     bool in[E];
 #pragma unroll
     for (int e = 0; e < E; ++e)
-        in[e] = column_of<VEC>(t, stride, e / 8, e % 8) < a.D;
+        in[e] = owns<WIDE>(t, stride, e / 8, e % 8, a.D);
 
     const bool branch = a.branch != nullptr, gated = branch && a.gate.data != nullptr;
-    Raw rr[NV], yr[NV];
+    const bool each = gated && a.gate_rows == 1;        // a gate for every element comes with the row
+    Raw rr[NV], yr[NV], gr[NV];
     auto load = [&](size_t row) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            rr[v] = load_raw<VEC>(a.residual, R, row * a.ld_residual, t, stride, v, a.D);
+            if (each)
+                gr[v] = load_raw<WIDE>(a.gate.data, a.gate.type, row * (size_t)a.D, t, stride, v, a.D);
+            rr[v] = load_raw<WIDE>(a.residual, R, row * a.ld_residual, t, stride, v, a.D);
             if (branch)
-                yr[v] = load_raw<VEC>(a.branch, T, row * a.ld_branch, t, stride, v, a.D);
+                yr[v] = load_raw<WIDE>(a.branch, T, row * a.ld_branch, t, stride, v, a.D);
         }
     };
     if (begin < end)
         load(begin);
-    Columns<VEC, NV, BIAS> p;
+    Columns<WIDE, NV, BIAS> p;
     size_t gate_row = begin / a.gate_rows;
-    p.load(a, gate_row, gated, t, stride);
+    p.load(a, gate_row, gated && !each, t, stride);
 
     for (size_t row = begin; row < end; ++row) {
         float s[E], mean, inv;
         float post_mean = 0.0f, post_inv = 1.0f, pre_mean = 0.0f, pre_inv = 1.0f;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
-            unpack<VEC>(rr[v], R, s + v * 8);
+            unpack(rr[v], R, s + v * 8);
         if (branch) {
             float y[E];
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                unpack<VEC>(yr[v], T, y + v * 8);
-            if (gated && row / a.gate_rows != gate_row) {
+                unpack(yr[v], T, y + v * 8);
+            if (each)
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+                    unpack(gr[v], a.gate.type, p.gate + v * 8);
+            else if (gated && row / a.gate_rows != gate_row) {
                 gate_row = row / a.gate_rows;
                 p.load_gate(a, gate_row, t, stride);
             }
             if (row + 1 < end)
                 load(row + 1);
             if (a.post != kNoNorm) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    y[e] = in[e] ? y[e] : 0.0f;
                 standardize<E>(y, in, a.post, inv_d, a.eps, sum, mean, inv);
                 post_mean = mean;
                 post_inv = inv;
@@ -347,11 +346,11 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
                 s[e] = fmaf(s[e], p.scale[e], y[e] * p.gate[e]);
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                store8<VEC>(a.sum, R, row * a.ld_sum, t, stride, v, a.D, s + v * 8);
+                store8<WIDE>(a.sum, R, row * a.ld_sum, t, stride, v, a.D, s + v * 8);
         } else if (row + 1 < end)
             load(row + 1);
         if (a.out) {
-            // columns beyond D: s may hold a bias there, it must not count
+            // (what is not its own must not count)
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 s[e] = in[e] ? s[e] : 0.0f;
@@ -365,7 +364,7 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
             }
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                store8<VEC>(a.out, T, row * a.ld_out, t, stride, v, a.D, s + v * 8);
+                store8<WIDE>(a.out, T, row * a.ld_out, t, stride, v, a.D, s + v * 8);
         }
         if (a.stats && t == 0)
             *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(post_mean, post_inv, pre_mean, pre_inv);
@@ -374,7 +373,7 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
 
 // ---- backward -----------------------------------------------------------------------------------------
 
-template <ElementType T, ElementType R, bool VEC, int NV, int THREADS, bool BIAS>
+template <ElementType T, ElementType R, bool WIDE, int NV, int THREADS, bool BIAS>
 __global__ void __launch_bounds__(THREADS)
 block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, int walkers, int per_gate, int gates_each)
 {
@@ -400,10 +399,15 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
     const float inv_d = 1.0f / (float)a.D;
     RowSum sum = {slots, 0, row_threads / 64};
     const bool branch = a.branch != nullptr, gated = branch && a.gate.data != nullptr;
+    bool in[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        in[e] = owns<WIDE>(t, stride, e / 8, e % 8, a.D);
 
-    Columns<VEC, NV, BIAS> p;
+    const bool each = gated && a.gate_rows == 1;        // a gate for every element comes with the row
+    Columns<WIDE, NV, BIAS> p;
     size_t gate_row = begin / a.gate_rows;
-    p.load(a, gate_row, gated, t, stride);
+    p.load(a, gate_row, gated && !each, t, stride);
     float sum_post_w[E], sum_scale[E], sum_pre_w[E], sum_gate[E], sum_post_b[BIAS ? E : 8], sum_pre_b[BIAS ? E : 8];
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -416,19 +420,21 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
     auto after = [&](float y, int e) { return BIAS ? fmaf(y, p.post_w[e], p.post_b[e]) : y * p.post_w[e]; };
 
     // the next row is on its way while one is worked on
-    Raw rr[NV], yr[NV], gs[NV], go[NV];
+    Raw rr[NV], yr[NV], gs[NV], go[NV], gr[NV];
     float4 stats = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     auto load = [&](size_t row) {
         stats = *reinterpret_cast<const float4*>(a.stats + row * 4);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            rr[v] = load_raw<VEC>(a.residual, R, row * a.ld_residual, t, stride, v, a.D);
+            if (each)
+                gr[v] = load_raw<WIDE>(a.gate.data, a.gate.type, row * (size_t)a.D, t, stride, v, a.D);
+            rr[v] = load_raw<WIDE>(a.residual, R, row * a.ld_residual, t, stride, v, a.D);
             if (branch)
-                yr[v] = load_raw<VEC>(a.branch, T, row * a.ld_branch, t, stride, v, a.D);
+                yr[v] = load_raw<WIDE>(a.branch, T, row * a.ld_branch, t, stride, v, a.D);
             if (d.sum)
-                gs[v] = load_raw<VEC>(d.sum, R, row * d.ld_sum, t, stride, v, a.D);
+                gs[v] = load_raw<WIDE>(d.sum, R, row * d.ld_sum, t, stride, v, a.D);
             if (d.out)
-                go[v] = load_raw<VEC>(d.out, T, row * d.ld_out, t, stride, v, a.D);
+                go[v] = load_raw<WIDE>(d.out, T, row * d.ld_out, t, stride, v, a.D);
         }
     };
     if (begin < end)
@@ -439,21 +445,26 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
             if (d.gate && per_gate == 1)
 #pragma unroll
                 for (int v = 0; v < NV; ++v)
-                    store8<VEC>(d.gate, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D, sum_gate + v * 8);
+                    store8<WIDE>(d.gate, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D, sum_gate + v * 8);
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 sum_gate[e] = 0.0f;
             gate_row = row / a.gate_rows;
-            p.load_gate(a, gate_row, t, stride);
+            if (!each)
+                p.load_gate(a, gate_row, t, stride);
         }
+        if (each)
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                unpack(gr[v], a.gate.type, p.gate + v * 8);
         float r[E], yn[E], s[E], ds[E], g[E];
 #pragma unroll
         for (int v = 0; v < NV; ++v)
-            unpack<VEC>(rr[v], R, r + v * 8);
+            unpack(rr[v], R, r + v * 8);
         if (branch) {
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                unpack<VEC>(yr[v], T, yn + v * 8);
+                unpack(yr[v], T, yn + v * 8);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 yn[e] = (yn[e] - st.x) * st.y;      // mean 0 and 1 / deviation 1 where there is no norm
@@ -466,7 +477,7 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
         if (d.sum)
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                unpack<VEC>(gs[v], R, ds + v * 8);
+                unpack(gs[v], R, ds + v * 8);
         else
 #pragma unroll
             for (int e = 0; e < E; ++e)
@@ -474,13 +485,14 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
         if (d.out)
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                unpack<VEC>(go[v], T, g + v * 8);   // zeros beyond D
+                unpack(go[v], T, g + v * 8);
         if (row + 1 < end)
             load(row + 1);
         if (d.out) {
             float with = 0.0f, plain = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
+                g[e] = in[e] ? g[e] : 0.0f;
                 s[e] = (s[e] - st.z) * st.w;
                 sum_pre_w[e] = fmaf(g[e], s[e], sum_pre_w[e]);
                 if (BIAS)
@@ -503,13 +515,13 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
             if (d.residual)
 #pragma unroll
                 for (int v = 0; v < NV; ++v)
-                    store8<VEC>(d.residual, R, row * d.ld_residual, t, stride, v, a.D, ds + v * 8);
+                    store8<WIDE>(d.residual, R, row * d.ld_residual, t, stride, v, a.D, ds + v * 8);
             continue;
         }
         float with = 0.0f, plain = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if (column_of<VEC>(t, stride, e / 8, e % 8) >= a.D)
+            if (!in[e])
                 ds[e] = 0.0f;
             sum_scale[e] = fmaf(ds[e], r[e], sum_scale[e]);
             sum_gate[e] = fmaf(ds[e], after(yn[e], e), sum_gate[e]);
@@ -525,7 +537,7 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
         if (d.residual)
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                store8<VEC>(d.residual, R, row * d.ld_residual, t, stride, v, a.D, r + v * 8);
+                store8<WIDE>(d.residual, R, row * d.ld_residual, t, stride, v, a.D, r + v * 8);
         if (a.post != kNoNorm) {
             sum(with, plain);
             with *= inv_d;
@@ -538,19 +550,19 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
         if (d.branch)
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                store8<VEC>(d.branch, T, row * d.ld_branch, t, stride, v, a.D, ds + v * 8);
+                store8<WIDE>(d.branch, T, row * d.ld_branch, t, stride, v, a.D, ds + v * 8);
     }
 
     if (gated && d.gate && per_gate == 1 && begin < end)
 #pragma unroll
         for (int v = 0; v < NV; ++v)
-            store8<VEC>(d.gate, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D, sum_gate + v * 8);
+            store8<WIDE>(d.gate, a.gate.type, gate_row * (size_t)a.D, t, stride, v, a.D, sum_gate + v * 8);
     // the walker's sums: [parameter][walker][column]
     auto leave = [&](int slot, const float* x) {
         if (slot >= 0)
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                store8<VEC>(d.partial, kF32, ((size_t)slot * walkers + walker) * a.D, t, stride, v, a.D, x + v * 8);
+                store8<WIDE>(d.partial, kF32, ((size_t)slot * walkers + walker) * a.D, t, stride, v, a.D, x + v * 8);
     };
     leave(d.slot_post_weight, sum_post_w);
     if (BIAS)
@@ -614,50 +626,43 @@ int row_threads_of(int D)
     return (((D + each - 1) / each) + 63) / 64 * 64;
 }
 
-bool vector_rows(const void* p, size_t ld, int D)
-{
-    return !p || ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0 && D % 8 == 0);
-}
-
-bool vector_forward(const BlockNormArgs& a)
-{
-    const size_t D = a.D;
-    return vector_rows(a.residual, a.ld_residual, a.D) && vector_rows(a.branch, a.ld_branch, a.D) && vector_rows(a.sum, a.ld_sum, a.D) &&
-           vector_rows(a.out, a.ld_out, a.D) && vector_rows(a.gate.data, D, a.D) && vector_rows(a.scale.data, D, a.D) &&
-           vector_rows(a.post_weight.data, D, a.D) && vector_rows(a.post_bias.data, D, a.D) &&
-           vector_rows(a.pre_weight.data, D, a.D) && vector_rows(a.pre_bias.data, D, a.D);
-}
-
-template <ElementType T, ElementType R, bool VEC>
+template <ElementType T, ElementType R>
 void forward(const BlockNormArgs& a, hipStream_t stream)
 {
     const int rt = row_threads_of(a.D), each = rt == 64 ? 4 : 1;
     // as many walkers as the GPU holds waves of this many registers (16 a compute unit)
     const size_t most = (size_t)machine().cus * 16 / (rt / 64);
-    const int walkers = (int)(a.rows < most ? a.rows : most);
+    const size_t turns = (a.rows + most - 1) / most;       // rows of a walker, the same for nearly all
+    const int walkers = (int)((a.rows + turns - 1) / turns);
     const dim3 grid((walkers + each - 1) / each), block(rt * each);
     const bool bias = a.post_bias.data || a.pre_bias.data;
-    if (a.D <= 8 * kMaxThreads)
-        bias ? block_norm_kernel<T, R, VEC, 1, true><<<grid, block, 0, stream>>>(a, rt, walkers)
-             : block_norm_kernel<T, R, VEC, 1, false><<<grid, block, 0, stream>>>(a, rt, walkers);
+#define NMSPMM_FORWARD(WIDE, NV, BIAS) block_norm_kernel<T, R, WIDE, NV, BIAS><<<grid, block, 0, stream>>>(a, rt, walkers)
+    if (a.D < 8)
+        NMSPMM_FORWARD(false, 1, true);
+    else if (a.D <= 8 * kMaxThreads)
+        bias ? NMSPMM_FORWARD(true, 1, true) : NMSPMM_FORWARD(true, 1, false);
     else
-        block_norm_kernel<T, R, VEC, 2, true><<<grid, block, 0, stream>>>(a, rt, walkers);
+        NMSPMM_FORWARD(true, 2, true);
+#undef NMSPMM_FORWARD
 }
 
-template <ElementType T, ElementType R, bool VEC>
+template <ElementType T, ElementType R>
 void backward(const BlockNormArgs& a, const BlockNormGrads& d, const BlockNormWalk& w, hipStream_t stream)
 {
     const int rt = row_threads_of(a.D), each = rt == 64 ? 4 : 1;
     const dim3 grid((w.walkers + each - 1) / each), block(rt * each);
     const bool bias = a.post_bias.data || a.pre_bias.data;
-#define NMSPMM_BACKWARD(NV, THREADS, BIAS) \
-    block_norm_backward_kernel<T, R, VEC, NV, THREADS, BIAS><<<grid, block, 0, stream>>>(a, d, rt, w.walkers, w.per_gate, w.gates_each)
-    if (a.D <= 4096)
-        bias ? NMSPMM_BACKWARD(1, 512, true) : NMSPMM_BACKWARD(1, 512, false);
+#define NMSPMM_BACKWARD(WIDE, NV, THREADS, BIAS)                                                                         \
+    block_norm_backward_kernel<T, R, WIDE, NV, THREADS, BIAS><<<grid, block, 0, stream>>>(a, d, rt, w.walkers, w.per_gate, \
+                                                                                          w.gates_each)
+    if (a.D < 8)
+        NMSPMM_BACKWARD(false, 1, 512, true);
+    else if (a.D <= 4096)
+        bias ? NMSPMM_BACKWARD(true, 1, 512, true) : NMSPMM_BACKWARD(true, 1, 512, false);
     else if (a.D <= 8 * kMaxThreads)
-        bias ? NMSPMM_BACKWARD(1, 1024, true) : NMSPMM_BACKWARD(1, 1024, false);
+        bias ? NMSPMM_BACKWARD(true, 1, 1024, true) : NMSPMM_BACKWARD(true, 1, 1024, false);
     else
-        NMSPMM_BACKWARD(2, 1024, true);
+        NMSPMM_BACKWARD(true, 2, 1024, true);
 #undef NMSPMM_BACKWARD
 }
 
@@ -665,8 +670,7 @@ void backward(const BlockNormArgs& a, const BlockNormGrads& d, const BlockNormWa
 
 hipError_t launch_block_norm(const BlockNormArgs& a, int type, int residual_type, hipStream_t stream)
 {
-    const bool vec = vector_forward(a);
-#define NMSPMM_TYPES(T, R) (vec ? forward<T, R, true>(a, stream) : forward<T, R, false>(a, stream))
+#define NMSPMM_TYPES(T, R) forward<T, R>(a, stream)
     if (type == kF32)
         NMSPMM_TYPES(kF32, kF32);
     else if (type == kBF16)
@@ -734,12 +738,8 @@ hipError_t launch_block_norm_backward(const BlockNormArgs& a, const BlockNormGra
         column(d.gate, a.gate.type, d.slot_gate);
         outputs += f.gates;
     }
-    const size_t D = a.D;
-    const bool vec = vector_forward(a) && vector_rows(d.sum, d.ld_sum, a.D) && vector_rows(d.out, d.ld_out, a.D) &&
-                     vector_rows(d.residual, d.ld_residual, a.D) && vector_rows(d.branch, d.ld_branch, a.D) &&
-                     vector_rows(d.gate, D, a.D);
     if (a.rows > 0) {
-#define NMSPMM_TYPES(T, R) (vec ? backward<T, R, true>(a, d, w, stream) : backward<T, R, false>(a, d, w, stream))
+#define NMSPMM_TYPES(T, R) backward<T, R>(a, d, w, stream)
         if (type == kF32)
             NMSPMM_TYPES(kF32, kF32);
         else if (type == kBF16)
