@@ -114,21 +114,26 @@ __device__ inline void store8(void* p, int type, size_t row, int t, int stride, 
     }
 }
 
-// The sum over a wave, in every lane: neighbours, quads and rows of 16 by lane permutation within the vector unit, rows and halves by
+// The sum over a row's lanes of a wave, in every one of them: neighbours, quads and rows of 16 by lane permutation within the vector unit, rows and halves by
 // swapping them (an exchange through LDS takes ten times as long, and a row waits for six of them in turn).
 template <int CTRL>
 __device__ inline float exchanged(float v)
 {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
 }
-__device__ inline float wave_sum(float v)
+// Rows of 16 or 32 lanes share a wave: theirs stop there.
+__device__ inline float lanes_sum(float v, int lanes)
 {
     v += exchanged<0xb1>(v);        // lane ^ 1
     v += exchanged<0x4e>(v);        // lane ^ 2
     v += exchanged<0x141>(v);       // the other quad of eight
     v += exchanged<0x140>(v);       // the other half of sixteen
+    if (lanes == 16)
+        return v;
     const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     v = __uint_as_float(rows[0]) + __uint_as_float(rows[1]);
+    if (lanes == 32)
+        return v;
     const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
 }
@@ -136,13 +141,13 @@ __device__ inline float wave_sum(float v)
 // Sums over the threads of a row: a wave, or the workgroup's waves through LDS (two halves used in turn: one barrier a sum).
 struct RowSum {
     float (*slots)[2][kMaxThreads / 64];
-    int half, waves;
+    int half, waves, lanes;
     template <bool BOTH>
     __device__ void add(float& a, float& b)
     {
-        a = wave_sum(a);
+        a = lanes_sum(a, lanes);
         if (BOTH)
-            b = wave_sum(b);
+            b = lanes_sum(b, lanes);
         if (waves == 1)
             return;
         if ((threadIdx.x & 63) == 0) {
@@ -270,8 +275,8 @@ private:
 
 // ---- forward ------------------------------------------------------------------------------------------
 
-template <ElementType T, ElementType R, bool WIDE, int NV, bool BIAS>
-__global__ void __launch_bounds__(kMaxThreads)
+template <ElementType T, ElementType R, bool WIDE, int NV, int THREADS, bool BIAS>
+__global__ void __launch_bounds__(THREADS)
 block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
 {
     __shared__ __attribute__((aligned(16))) float slots[2][2][kMaxThreads / 64];
@@ -279,12 +284,12 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
     constexpr int E = NV * 8;
     const int t = threadIdx.x % row_threads;
     const int walker = blockIdx.x * (blockDim.x / row_threads) + threadIdx.x / row_threads;
-    if (walker >= walkers)      // whole waves, and only where a row is one wave: no barrier is missed
+    if (walker >= walkers)      // only where a row is a wave or a part of one: no barrier is missed
         return;
     const size_t begin = (size_t)walker * a.rows / walkers, end = (size_t)(walker + 1) * a.rows / walkers;
     const int stride = row_threads;
     const float inv_d = 1.0f / (float)a.D;
-    RowSum sum = {slots, 0, row_threads / 64};
+    RowSum sum = {slots, 0, (row_threads + 63) / 64, min(row_threads, 64)};
     bool in[E];
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -397,7 +402,7 @@ block_norm_backward_kernel(BlockNormArgs a, BlockNormGrads d, int row_threads, i
     }
     const int stride = row_threads;
     const float inv_d = 1.0f / (float)a.D;
-    RowSum sum = {slots, 0, row_threads / 64};
+    RowSum sum = {slots, 0, (row_threads + 63) / 64, min(row_threads, 64)};
     const bool branch = a.branch != nullptr, gated = branch && a.gate.data != nullptr;
     bool in[E];
 #pragma unroll
@@ -619,9 +624,11 @@ block_norm_finish_kernel(FinishArgs f)
     }
 }
 
-// Threads of a row, in whole waves: 8 elements each up to 8192 features, 16 beyond.
+// Threads of a row, 8 elements each up to 8192 features, 16 beyond: whole waves, or 16 or 32 lanes of one.
 int row_threads_of(int D)
 {
+    if (D <= 256)
+        return D <= 128 ? 16 : 32;
     const int each = D <= 8 * kMaxThreads ? 8 : 16;
     return (((D + each - 1) / each) + 63) / 64 * 64;
 }
@@ -629,34 +636,36 @@ int row_threads_of(int D)
 template <ElementType T, ElementType R>
 void forward(const BlockNormArgs& a, hipStream_t stream)
 {
-    const int rt = row_threads_of(a.D), each = rt == 64 ? 4 : 1;
+    const int rt = row_threads_of(a.D), each = rt <= 64 ? 256 / rt : 1;
     // as many walkers as the GPU holds waves of this many registers (16 a compute unit)
-    const size_t most = (size_t)machine().cus * 16 / (rt / 64);
+    const size_t most = (size_t)machine().cus * 16 * 64 / rt;
     const size_t turns = (a.rows + most - 1) / most;       // rows of a walker, the same for nearly all
     const int walkers = (int)((a.rows + turns - 1) / turns);
     const dim3 grid((walkers + each - 1) / each), block(rt * each);
     const bool bias = a.post_bias.data || a.pre_bias.data;
-#define NMSPMM_FORWARD(WIDE, NV, BIAS) block_norm_kernel<T, R, WIDE, NV, BIAS><<<grid, block, 0, stream>>>(a, rt, walkers)
+#define NMSPMM_FORWARD(WIDE, NV, THREADS, BIAS) block_norm_kernel<T, R, WIDE, NV, THREADS, BIAS><<<grid, block, 0, stream>>>(a, rt, walkers)
     if (a.D < 8)
-        NMSPMM_FORWARD(false, 1, true);
+        NMSPMM_FORWARD(false, 1, 256, true);
+    else if (bias && a.D <= 4096)
+        NMSPMM_FORWARD(true, 1, 512, true);
     else if (a.D <= 8 * kMaxThreads)
-        bias ? NMSPMM_FORWARD(true, 1, true) : NMSPMM_FORWARD(true, 1, false);
+        bias ? NMSPMM_FORWARD(true, 1, 1024, true) : NMSPMM_FORWARD(true, 1, 1024, false);
     else
-        NMSPMM_FORWARD(true, 2, true);
+        NMSPMM_FORWARD(true, 2, 1024, true);
 #undef NMSPMM_FORWARD
 }
 
 template <ElementType T, ElementType R>
 void backward(const BlockNormArgs& a, const BlockNormGrads& d, const BlockNormWalk& w, hipStream_t stream)
 {
-    const int rt = row_threads_of(a.D), each = rt == 64 ? 4 : 1;
+    const int rt = row_threads_of(a.D), each = rt <= 64 ? 256 / rt : 1;
     const dim3 grid((w.walkers + each - 1) / each), block(rt * each);
     const bool bias = a.post_bias.data || a.pre_bias.data;
 #define NMSPMM_BACKWARD(WIDE, NV, THREADS, BIAS)                                                                         \
     block_norm_backward_kernel<T, R, WIDE, NV, THREADS, BIAS><<<grid, block, 0, stream>>>(a, d, rt, w.walkers, w.per_gate, \
                                                                                           w.gates_each)
     if (a.D < 8)
-        NMSPMM_BACKWARD(false, 1, 512, true);
+        NMSPMM_BACKWARD(false, 1, 256, true);
     else if (a.D <= 4096)
         bias ? NMSPMM_BACKWARD(true, 1, 512, true) : NMSPMM_BACKWARD(true, 1, 512, false);
     else if (a.D <= 8 * kMaxThreads)
@@ -685,8 +694,8 @@ hipError_t launch_block_norm(const BlockNormArgs& a, int type, int residual_type
 // walker with a part of a gate's rows beside rows of another gate.
 BlockNormWalk block_norm_walk(long long rows, long long gate_rows, int D)
 {
-    const int waves = row_threads_of(D) / 64;
-    const long long most = (long long)machine().cus * 16 / (waves < 8 ? waves : 8);
+    const int threads = row_threads_of(D);
+    const long long most = (long long)machine().cus * 16 * 64 / (threads < 512 ? threads : 512);
     long long rows_each = (rows + most - 1) / most;
     if (rows_each < 4)
         rows_each = 4;
