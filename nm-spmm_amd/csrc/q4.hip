@@ -8,8 +8,8 @@
 // blocks of 128 kept rows x 16 columns, 1 KB each, ordered by column tile, then block.
 //   codes [tile][block][lane][4] uint32: lane 16 kb + c holds column c, word s its rows
 //         32 s + 8 kb + 0..7 (a k-step of 32 rows of a matrix instruction); nibble i of the word is row
-//         2 i of the eight, nibble i + 4 row 2 i + 1, so that the words of the operand registers come
-//         out of one shift and one mask-and-or each.
+//         2 i of the eight, nibble i + 4 row 2 i + 1, and the whole is rotated left by three bits, so that the
+//         operand registers come out of one shift (the first: none) and one mask-and-or each.
 //   meta  [tile][block][16 columns][128 / group] uint32: the scale's fp32 bits with the zero point in
 //         the low four.
 //   rows  [N / 32][blocks * 128] uint8 (n < m only): the dense row of each kept row, counted from the
@@ -226,7 +226,7 @@ q4_pack_kernel(const float* __restrict__ values, const uint8_t* __restrict__ giv
         }
         const uint32_t mask = FROM_VALUES && !(scale > 0.0f) ? 0u : in;     // (nothing counts under a scale of 0 or NaN)
         w = (w & mask) | ((mt[i] & 15u) * 0x11111111u & ~mask);
-        words[kb * Cols + c * V + i][s] = w;
+        words[kb * Cols + c * V + i][s] = __builtin_amdgcn_alignbit(w, w, 29);
         if (kb == 0)
             groups[g][c * V + i] = mt[i];
     }
@@ -289,9 +289,10 @@ q4_expand_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict_
             const uint32_t m = per == 4 ? mt[i][s] : per == 2 ? mt[i][s >> 1] : mt[i][0];
             const float scale = __uint_as_float(m & ~15u);
             const int zero = (int)(m & 15u);
+            const uint32_t packed = __builtin_amdgcn_alignbit(word[i][s], word[i][s], 3);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                v[e][i] = scale * (float)((int)((word[i][s] >> nibble(e)) & 15u) - zero);
+                v[e][i] = scale * (float)((int)((packed >> nibble(e)) & 15u) - zero);
         }
         const int r0 = block * 128 + s * 32 + kb * 8;
         if (KEPT == 0) {

@@ -29,14 +29,15 @@ __device__ inline uint32_t sixteens()
     return one;
 }
 
-// Eight codes -> eight operand elements 16 + code.
+// Eight codes -> eight operand elements 16 + code (a word's bits are rotated so that the first pair is in place for bf16: q4.hip).
 template <ElementType T>
 __device__ inline u32x4 widened(uint32_t w, uint32_t one)
 {
     const uint32_t mask = T == kF16 ? 0x03c003c0u : 0x00780078u;
     if (T == kF16)
-        return u32x4{((w << 6) & mask) | one, ((w << 2) & mask) | one, ((w >> 2) & mask) | one, ((w >> 6) & mask) | one};
-    return u32x4{((w << 3) & mask) | one, ((w >> 1) & mask) | one, ((w >> 5) & mask) | one, ((w >> 9) & mask) | one};
+        return u32x4{((w << 3) & mask) | one, ((w >> 1) & mask) | one, ((w >> 5) & mask) | one,
+                     (__builtin_amdgcn_alignbit(w, w, 9) & mask) | one};
+    return u32x4{(w & mask) | one, ((w >> 4) & mask) | one, ((w >> 8) & mask) | one, (__builtin_amdgcn_alignbit(w, w, 12) & mask) | one};
 }
 
 template <ElementType T>

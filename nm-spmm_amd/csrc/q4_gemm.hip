@@ -98,7 +98,8 @@ q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict
         const int r0 = d0 / p.m * p.n;                                      // a multiple of KEPT: all in one word
         const size_t at = (size_t)tile * p.blocks + (r0 >> 7);
         const uint32_t zero = meta[(at * 16 + c) * per + ((r0 >> 5) & 3) * per / 4] & 15u;
-        const uint32_t packed = codes[(at * 64 + ((r0 >> 3) & 3) * 16 + c) * 4 + ((r0 >> 5) & 3)];
+        const uint32_t rotated = codes[(at * 64 + ((r0 >> 3) & 3) * 16 + c) * 4 + ((r0 >> 5) & 3)];
+        const uint32_t packed = __builtin_amdgcn_alignbit(rotated, rotated, 3);
         const uint2 eight = *reinterpret_cast<const uint2*>(rows + (size_t)(tile >> 1) * p.blocks * 128 + (r0 & ~7));
         const int base = (r0 >> 5) * p.span - d0;
         uint32_t dense = zero * 0x11111111u;
@@ -111,7 +112,7 @@ q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict
             const uint32_t change = ((packed >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) ^ zero;
             dense ^= d < 8u && r0 + i < p.W ? change << (2 * (d & 6) + 16 * (d & 1)) : 0u;
         }
-        word[s] = dense;
+        word[s] = __builtin_amdgcn_alignbit(dense, dense, 29);
     }
     *reinterpret_cast<u32x4*>(out + (((size_t)tile * dense_blocks + block) * 64 + lane) * 4) = word;
 }
