@@ -33,9 +33,17 @@ __device__ inline __amdgpu_buffer_rsrc_t window(const void* base, size_t bytes)
 // A workgroup takes NC 16-column tiles and at most RT row tiles; its waves take the blocks of 128 kept rows in turn
 // and add up their sums in LDS at the end, in wave order.  A block costs about 60 vector instructions a tile, which is what bounds
 // the kernel beside the launch: addresses are scalars, ends are left to the descriptors' bounds, groups are unrolled.
-// MX: rows of x the instance has registers for; UNITS: scaled groups in a block; the next DEPTH blocks are on their way.
+// MX: rows of x the instance has registers for; UNITS: scaled groups in a block.
 // What an instance needs registers for decides how many waves it runs with.
 constexpr int most_waves(int RT, int MX) { return MX > 8 || (RT > 1 && MX == 1) ? kMaxWaves / 2 : kMaxWaves; }
+
+// Blocks under way at a time.
+constexpr int depth_of(Source src, int RT, int NC, int MX, int UNITS)
+{
+    if (src == kDirect)
+        return RT == 1 && NC == 1 && UNITS < 4 ? 3 : 2;
+    return MX == 1 ? (NC == 1 ? 4 : UNITS < 4 ? 3 : 2) : MX == 4 && NC == 1 ? 3 : 2;
+}
 
 template <ElementType T, Source SRC, int RT, int NC, int MX, int UNITS>
 __global__ void __launch_bounds__(most_waves(RT, MX) * 64)
@@ -203,28 +211,27 @@ q4_rows_product_kernel(const void* __restrict__ x_, size_t ldx, const uint32_t* 
         }
     };
 
-    // two blocks' loads are under way at any time (a gathered x one block behind its places)
-    Block one, two;
-    if (wave < p.blocks)
-        load(wave, one);
-    if (wave + waves < p.blocks)
-        load(wave + waves, two);
+    // DEPTH blocks' loads are under way at any time (a gathered x one block behind its places)
+    constexpr int DEPTH = depth_of(SRC, RT, NC, MX, UNITS);
+    Block blocks[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (wave + d * waves < p.blocks)
+            load(wave + d * waves, blocks[d]);
     if (SRC == kGathered && wave < p.blocks)
-        gather(wave, one);
-    for (int b = wave; b < p.blocks; b += 2 * waves) {
-        if (SRC == kGathered && b + waves < p.blocks)
-            gather(b + waves, two);
-        multiply(one);
-        if (b + 2 * waves < p.blocks)
-            load(b + 2 * waves, one);
-        if (b + waves >= p.blocks)
-            break;
-        if (SRC == kGathered && b + 2 * waves < p.blocks)
-            gather(b + 2 * waves, one);
-        multiply(two);
-        if (b + 3 * waves < p.blocks)
-            load(b + 3 * waves, two);
-    }
+        gather(wave, blocks[0]);
+    for (int first = wave; first < p.blocks; first += DEPTH * waves)
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const int b = first + d * waves;
+            if (b >= p.blocks)
+                break;
+            if (SRC == kGathered && b + waves < p.blocks)
+                gather(b + waves, blocks[(d + 1) % DEPTH]);
+            multiply(blocks[d]);
+            if (b + DEPTH * waves < p.blocks)
+                load(b + DEPTH * waves, blocks[d]);
+        }
 
     // the waves' sums: [wave][row][column]; an fp32 row is the sum of its three pieces, smallest first
     float* const part = reinterpret_cast<float*>(lds);
