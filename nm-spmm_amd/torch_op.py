@@ -145,15 +145,10 @@ def _guard(tensor):
     return torch.cuda.device(tensor.device)
 
 
-def _on_device(call, index, *args):
-    """call(*args, the device's current stream), with that device as the current one; raises what the status says."""
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            status = call(*args, _stream_of(index))
-    else:
-        status = call(*args, _stream_of(index))
+def _call(function, *args):
+    status = function(*args)
     if status != _nm.OK:
-        raise _nm.NmSpmmError(call.__name__, status)
+        raise _nm.NmSpmmError(function.__name__, status)
 
 
 class NMQuantOperand:
@@ -207,8 +202,8 @@ class NMQuantOperand:
         per_group = (-(-codes.shape[0] // group), codes.shape[1])
         if scale.shape != per_group or scale.device != codes.device or not scale.is_floating_point():
             raise ValueError("scale must be a floating tensor %s on the device of the codes" % (per_group,))
-        if zero is not None and (zero.shape != per_group or zero.device != codes.device):
-            raise ValueError("zero must be a tensor %s on the device of the codes" % (per_group,))
+        if zero is not None and (zero.shape != per_group or zero.device != codes.device or zero.is_floating_point()):
+            raise ValueError("zero must be a tensor %s of whole numbers 0..15 on the device of the codes" % (per_group,))
         rows = operand._rows(rows, codes)
         with _guard(codes):
             _nm.q4_pack_device(codes.contiguous(), scale.to(torch.float32).contiguous(),
@@ -228,6 +223,10 @@ def _quant_linear(x, operand):
     K, N = operand.K, operand.N
     if x.shape[-1] != K or x.dtype not in _TYPES or not x.is_cuda:
         raise ValueError("x must be a float32, bfloat16 or float16 CUDA tensor whose last dimension is %d" % K)
+    index = x.get_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _quant_linear(x, operand)
     y = x.new_empty((*x.shape[:-1], N))
     M = y.numel() // N
     if M == 0:
@@ -245,7 +244,7 @@ def _quant_linear(x, operand):
         if need:
             workspace = x.new_empty(need, dtype=torch.uint8)    # from torch's caching allocator, ordered on the stream
             space = workspace.data_ptr()
-    _on_device(lib.nmspmm_q4_linear, x.get_device(), operand, x.data_ptr(), ldx, y.data_ptr(), N, M, type_, space, need)
+    _call(lib.nmspmm_q4_linear, operand, x.data_ptr(), ldx, y.data_ptr(), N, M, type_, space, need, _stream_of(index))
     return y
 
 
@@ -385,19 +384,28 @@ def _pack_block_norm(residual, branch, total, out, stats, params, factor, post, 
 
 def _block_norm_forward(residual, branch, params, factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out, want_stats):
     """(sum or None, out or None, stats or None)."""
+    index = residual.get_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _block_norm_forward(residual, branch, params, factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out, want_stats)
     total = None if branch is None else residual.new_empty(residual.shape)
     out = residual.new_empty(residual.shape, dtype=dtype) if want_out else None
     stats = residual.new_empty((residual.numel() // residual.shape[-1], 4), dtype=torch.float32) if want_stats else None
     if residual.numel() == 0:
         return total, out, stats
     packed, keep = _pack_block_norm(residual, branch, total, out, stats, params, factor, post, pre, eps, weight_offset, gate_rows, dtype)
-    _on_device(_nm.lib().nmspmm_block_norm_forward, residual.get_device(), packed)
+    _call(_nm.lib().nmspmm_block_norm_forward, packed, _stream_of(index))
     return total, out, stats
 
 
 def _block_norm_backward(residual, branch, params, stats, grad_sum, grad_out, factor, post, pre, eps, weight_offset, gate_rows,
                          dtype, want_out, needs):
     """Gradients of (residual, branch, *params), None where `needs` is false or there is no such input."""
+    index = residual.get_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _block_norm_backward(residual, branch, params, stats, grad_sum, grad_out, factor, post, pre, eps, weight_offset,
+                                        gate_rows, dtype, want_out, needs)
     D = residual.shape[-1]
     given = (residual, branch, *params)
     if residual.numel() == 0:
@@ -415,7 +423,7 @@ def _block_norm_backward(residual, branch, params, stats, grad_sum, grad_out, fa
     lib = _nm.lib()
     need = lib.nmspmm_block_norm_workspace_bytes(residual.numel() // D, gate_rows, D)
     workspace = residual.new_empty(need // 4, dtype=torch.float32)
-    _on_device(lib.nmspmm_block_norm_backward, residual.get_device(), packed, want, workspace.data_ptr(), need)
+    _call(lib.nmspmm_block_norm_backward, packed, want, workspace.data_ptr(), need, _stream_of(index))
     return grads
 
 
@@ -534,7 +542,8 @@ def block_norm(residual, branch=None, *, gate=None, residual_scale=1.0, post=Non
     branch ([D], [batch, 1, D], a whole [batch, tokens, D], ...); residual_scale is a number or a tensor [D] (or of one element); weights and
     biases are [D], weight_offset is added to the weights.  residual is float32 or of branch's type; `dtype` is out's type
     (branch's where there is one, else residual's unless given).  All arithmetic is float32.  Differentiable once with respect to every
-    tensor; gradients repeat bit for bit.
+    tensor; gradients repeat bit for bit.  (As with any torch operator, capture a backward pass into a graph only while no eager
+    autograd graph over the same leaves is alive.)
     """
     if not residual.is_cuda or residual.dtype not in _TYPES or residual.dim() < 1:
         raise ValueError("residual must be a float32, bfloat16 or float16 CUDA tensor")

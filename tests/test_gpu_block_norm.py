@@ -373,7 +373,7 @@ def test_graph_replays_forward_and_backward():
 
     def step():
         total, out = call(dict(t, **leaves), conf, dt)
-        return (total, out, *torch.autograd.grad((total, out), list(leaves.values()), (gs, go)))
+        return (total.detach(), out.detach(), *torch.autograd.grad((total, out), list(leaves.values()), (gs, go)))
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -418,6 +418,26 @@ def test_registered_operators_trace_and_match():
     traced = torch.autograd.grad(sum(x.square().sum() for x in torch.compile(f, fullgraph=True, backend="aot_eager")(*leaves)), leaves)
     for a, b in zip(traced, eager):
         torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-5)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows whose elements lie beyond 4 GiB, forward and backward: the last are those of a small call."""
+    rows, D = 290000, 8192
+    r, y = (torch.zeros((rows, D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    tail = [torch.randn((5, D), device="cuda").bfloat16() for _ in range(2)]
+    r[-5:], y[-5:] = tail
+    w = torch.randn(D, device="cuda")
+    gs = torch.ones((5, D), dtype=torch.bfloat16, device="cuda")
+
+    def f(a, b, d):
+        a, b = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        total, out = op().block_norm(a, b, post="rms", post_weight=w, pre_weight=w)
+        return (total.detach(), out.detach(), *torch.autograd.grad((total, out), (a, b), (d, d)))
+
+    full = torch.zeros((rows, D), dtype=torch.bfloat16, device="cuda")
+    full[-5:] = gs
+    for got, want in zip(f(r, y, full), f(*tail, gs)):
+        assert torch.equal(got[-5:], want) and not bool(got[:-5].any())
 
 
 def test_refusals():

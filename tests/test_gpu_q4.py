@@ -331,18 +331,19 @@ def test_registered_operator_traces_and_matches():
     torch.library.opcheck(op().quant_linear, (x, layer.codes, layer.scales, None, layer.bias, 256, 64, 1, 1, 128))
 
 
-@pytest.mark.parametrize("M,n,m", [(1, 1, 1), (1, 2, 8), (24, 1, 1), (24, 2, 8), (150, 1, 1), (150, 2, 4)])
-def test_graph_replays(M, n, m):
-    made = make(12, 512, 128, n, m)
-    layer = layer_of(made, 512, n, m)
-    x = torch.randn((M, 512), device="cuda", dtype=torch.bfloat16)
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("M,n,m", [(1, 1, 1), (1, 2, 8), (12, 1, 1), (12, 2, 8), (24, 1, 1), (24, 2, 8), (150, 1, 1), (150, 2, 4)])
+def test_graph_replays(M, n, m, dtype):
+    made = make(12, 2048, 128, n, m)
+    layer = layer_of(made, 2048, n, m)
+    x = torch.randn((M, 2048), device="cuda", dtype=DTYPES[dtype])
     layer(x)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         y = layer(x)
     for k in range(4):
-        x.copy_(torch.randn((M, 512), device="cuda"))
+        x.copy_(torch.randn((M, 2048), device="cuda"))
         want = layer(x)
         graph.replay()
         torch.cuda.synchronize()
@@ -366,6 +367,33 @@ def test_two_streams_and_repeats_agree_bit_for_bit():
         assert torch.equal(y, want[k % len(want)])
 
 
+def test_offsets_beyond_32_bits():
+    """x of more than 4 GiB: its last rows are multiplied like any others, the zeros before them give zeros.  Codes of more than 4 GiB (K 2^17, N 2^16 and a bit): the
+    last columns are those of an operand that holds only them."""
+    made = make(30, 8192, 96)
+    layer = layer_of(made, 8192)
+    M = 280000
+    x = torch.zeros((M, 8192), dtype=torch.bfloat16, device="cuda")
+    tail = torch.randn((70, 8192), device="cuda").bfloat16()
+    x[-70:] = tail
+    y = layer(x)
+    assert not bool(y[:-70].any())
+    check(y[-70:], tail, made, 128)
+    del x, y
+    K, N = 1 << 17, (1 << 16) + 64
+    codes = torch.randint(0, 16, (K, N), dtype=torch.uint8, device="cuda")
+    scale = torch.rand((K // 128, N), device="cuda").half().float()
+    layer = op().NMQuantLinear.from_codes(codes, scale, None, K)
+    small = op().NMQuantLinear.from_codes(codes[:, -128:].contiguous(), scale[:, -128:].contiguous(), None, K)
+    del codes, scale
+    for M, dtype in ((1, torch.float32), (3, torch.bfloat16), (100, torch.float16)):
+        x = torch.randn((M, K), device="cuda").to(dtype)
+        got, want = layer(x)[:, -128:].double(), small(x).double()
+        # other waves and ranges of K may take the blocks: fp32 sums in another order, each below 1e-5 of its norm
+        half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps
+        assert float((got - want).norm()) <= (2e-5 + half) * float(want.norm())
+
+
 def test_refusals():
     layer = layer_of(make(13, 256, 64), 256)
     x = torch.randn((2, 256), device="cuda")
@@ -383,6 +411,8 @@ def test_refusals():
         op().NMQuantOperand.from_codes(cuda(codes), cuda(scale)[:1], None, 256, group=128)
     with pytest.raises(ValueError):
         op().NMQuantOperand.from_codes(cuda(codes).int(), cuda(scale), None, 256)
+    with pytest.raises(ValueError):
+        op().NMQuantOperand.from_codes(cuda(codes), cuda(scale), cuda(scale), 256)       # a zero point that is no whole number
     with pytest.raises(ValueError):
         op().NMQuantOperand.from_codes(cuda(codes), cuda(scale), None, 512, n=1, m=2)     # no rows
     with pytest.raises(ValueError):
