@@ -10,6 +10,8 @@ The reference has no framework binding; its driver multiplies synthetic operands
 (tests/test_nmspmm.cu:72-97).  The sequence of calls here is that driver's, on real weights.
 """
 import importlib
+import importlib.util
+import os
 from typing import List, Optional, Tuple
 
 import torch
@@ -133,22 +135,28 @@ class NMSparseLinear(torch.nn.Module):
 
 # ---- operands in 4 bits -----------------------------------------------------------------------------
 
-_TYPES = {torch.float32: _nm.F32, torch.bfloat16: _nm.BF16, torch.float16: _nm.F16}
+_native = None
 
 
-# the current stream of a device, by its index, as an integer (without a Stream object, which takes longer than a launch)
-_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+def _binding():
+    """csrc/torch_binding.cpp, built beside the library; raises if it has not been (no silent fallback)."""
+    global _native
+    if _native is None:
+        _nm.lib()
+        path = os.path.join(os.path.dirname(_nm.LIB_PATH), "_torch_binding.so")
+        if not os.path.exists(path):
+            raise RuntimeError("_torch_binding.so is not built: run `make -C %s` (or __graft_entry__.build())" % _nm.CSRC_DIR)
+        spec = importlib.util.spec_from_file_location(__name__.rsplit(".", 1)[0] + "._torch_binding", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.set_error(_nm.NmSpmmError)
+        _native = module
+    return _native
 
 
 def _guard(tensor):
     """Makes the tensor's device the current one (kernels are launched there)."""
     return torch.cuda.device(tensor.device)
-
-
-def _call(function, *args):
-    status = function(*args)
-    if status != _nm.OK:
-        raise _nm.NmSpmmError(function.__name__, status)
 
 
 class NMQuantOperand:
@@ -218,46 +226,11 @@ class NMQuantOperand:
         return out
 
 
-def _quant_linear(x, operand):
-    """x [..., K] times the operand of the struct (its bias added): [..., N] of x's type."""
-    K, N = operand.K, operand.N
-    if x.shape[-1] != K or x.dtype not in _TYPES or not x.is_cuda:
-        raise ValueError("x must be a float32, bfloat16 or float16 CUDA tensor whose last dimension is %d" % K)
-    index = x.get_device()
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return _quant_linear(x, operand)
-    y = x.new_empty((*x.shape[:-1], N))
-    M = y.numel() // N
-    if M == 0:
-        return y
-    ldx = K
-    if not x.is_contiguous():
-        x = x.reshape(M, K)
-        ldx = x.stride(0) if M > 1 else K
-        if (K > 1 and x.stride(1) != 1) or ldx < K or ldx > 1 << 24:
-            x, ldx = x.contiguous(), K
-    type_, need, space = _TYPES[x.dtype], 0, None
-    lib = _nm.lib()
-    if M > 8:       # below, no operand needs a workspace
-        need = lib.nmspmm_q4_workspace_bytes(M, K, N, operand.n, operand.m, type_)
-        if need:
-            workspace = x.new_empty(need, dtype=torch.uint8)    # from torch's caching allocator, ordered on the stream
-            space = workspace.data_ptr()
-    _call(lib.nmspmm_q4_linear, operand, x.data_ptr(), ldx, y.data_ptr(), N, M, type_, space, need, _stream_of(index))
-    return y
-
-
 @torch.library.custom_op("nmspmm::quant_linear", mutates_args=(), device_types="cuda")
 def quant_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, row_offsets: Optional[torch.Tensor],
                  bias: Optional[torch.Tensor], K: int, N: int, n: int, m: int, group: int) -> torch.Tensor:
     """x [..., K] row-major times an operand in 4 bits (NMQuantOperand) plus a float32 bias: [..., N] of x's type."""
-    for t in (codes, scales, row_offsets, bias):
-        if t is not None and (t.device != x.device or not t.is_contiguous()):
-            raise ValueError("the operand's buffers and the bias must be contiguous and on the device of x")
-    if bias is not None:
-        bias = bias.to(torch.float32)
-    return _quant_linear(x, _nm.q4_operand(codes, scales, row_offsets, K, N, n, m, group, bias))
+    return _binding().quant_linear(x, codes, scales, row_offsets, bias, K, N, n, m, group)
 
 
 @quant_linear.register_fake
@@ -310,18 +283,8 @@ class NMQuantLinear(torch.nn.Module):
         self.register_buffer("bias", None if bias is None else bias.detach().to(torch.float32).contiguous())
 
     def _operand(self):
-        # the struct of device pointers is kept between calls and follows the buffers
         b = self._buffers
-        codes, scales, rows, bias = b["codes"], b["scales"], b["row_offsets"], b["bias"]
-        at = (codes.data_ptr(), scales.data_ptr(), None if rows is None else rows.data_ptr(), None if bias is None else bias.data_ptr())
-        kept = self.__dict__.get("_struct")
-        if kept is None or kept[0] != at:
-            kept = (at, _nm.q4_operand(codes, scales, rows, self.in_features, self.out_features, self.n, self.m, self.group, bias))
-            self.__dict__["_struct"] = kept
-        return kept[1]
-
-    def __getstate__(self):
-        return {k: v for k, v in self.__dict__.items() if k != "_struct"}
+        return _nm.q4_operand(b["codes"], b["scales"], b["row_offsets"], self.in_features, self.out_features, self.n, self.m, self.group, b["bias"])
 
     def dense_weight(self):
         """The weight as a dense float32 [out_features, in_features] tensor."""
@@ -333,12 +296,10 @@ class NMQuantLinear(torch.nn.Module):
     def forward(self, x):
         b = self._buffers
         bias, codes = b["bias"], b["codes"]
-        # eager inference on the layer's device goes straight to the library; tracing, gradients and
-        # layers that were cast go through the registered operator
-        if type(x) is torch.Tensor and not torch.compiler.is_compiling() and x.device == codes.device and \
-                (bias is None or bias.dtype is torch.float32) and not (x.requires_grad and torch.is_grad_enabled()):
-            return _quant_linear(x, self._operand())
-        return quant_linear(x, codes, b["scales"], b["row_offsets"], bias, self.in_features, self.out_features, self.n, self.m, self.group)
+        # eager inference goes straight to the binding; tracing and gradients see the registered operator
+        eager = type(x) is torch.Tensor and not torch.compiler.is_compiling() and not (x.requires_grad and torch.is_grad_enabled())
+        return (_binding().quant_linear if eager else quant_linear)(
+            x, codes, b["scales"], b["row_offsets"], bias, self.in_features, self.out_features, self.n, self.m, self.group)
 
     def extra_repr(self):
         return "in_features=%d, out_features=%d, pattern=%d:%d, group=%d, bias=%s" % (
@@ -348,115 +309,17 @@ class NMQuantLinear(torch.nn.Module):
 # ---- the norms around a block -----------------------------------------------------------------------
 
 _NORMS = {None: _nm.NORM_NONE, "rms": _nm.NORM_RMS, "layer": _nm.NORM_LAYER}
-_PARAMS = ("gate", "residual_scale", "post_weight", "post_bias", "pre_weight", "pre_bias")
 
 
-def _as_rows(t, D):
-    """(t, elements between its rows): t itself where its leading dimensions can be walked as rows, else a copy."""
-    if t.is_contiguous():
-        return t, D
-    rows = t.reshape(-1, D)
-    if (D > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < D):
-        rows = rows.contiguous()
-    return rows, max(rows.stride(0), D)
-
-
-def _at(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _pack_block_norm(residual, branch, total, out, stats, params, factor, post, pre, eps, weight_offset, gate_rows, dtype):
-    """The packed struct, and the tensors (possibly copies) whose memory it names."""
-    D = residual.shape[-1]
-    rows = residual.numel() // D
-    residual, ld_residual = _as_rows(residual, D)
-    ld_branch = D
-    if branch is not None:
-        branch, ld_branch = _as_rows(branch, D)
-    gate, scale, post_w, post_b, pre_w, pre_b = params = [p if p is None or p.is_contiguous() else p.contiguous() for p in params]
-    packed = _nm.BLOCK_NORM.pack(
-        rows, gate_rows, ld_residual, ld_branch, D, D, residual.data_ptr(), _at(branch), _at(total), _at(out), _at(stats),
-        _at(gate), _at(scale), _at(post_w), _at(post_b), _at(pre_w), _at(pre_b),
-        *[0 if p is None else _TYPES[p.dtype] for p in params],
-        D, _TYPES[dtype], _TYPES[residual.dtype], post, pre, factor, eps, weight_offset)
-    return packed, (residual, branch, params)
-
-
-def _block_norm_forward(residual, branch, params, factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out, want_stats):
-    """(sum or None, out or None, stats or None)."""
-    index = residual.get_device()
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return _block_norm_forward(residual, branch, params, factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out, want_stats)
-    total = None if branch is None else residual.new_empty(residual.shape)
-    out = residual.new_empty(residual.shape, dtype=dtype) if want_out else None
-    stats = residual.new_empty((residual.numel() // residual.shape[-1], 4), dtype=torch.float32) if want_stats else None
-    if residual.numel() == 0:
-        return total, out, stats
-    packed, keep = _pack_block_norm(residual, branch, total, out, stats, params, factor, post, pre, eps, weight_offset, gate_rows, dtype)
-    _call(_nm.lib().nmspmm_block_norm_forward, packed, _stream_of(index))
-    return total, out, stats
-
-
-def _block_norm_backward(residual, branch, params, stats, grad_sum, grad_out, factor, post, pre, eps, weight_offset, gate_rows,
-                         dtype, want_out, needs):
-    """Gradients of (residual, branch, *params), None where `needs` is false or there is no such input."""
-    index = residual.get_device()
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return _block_norm_backward(residual, branch, params, stats, grad_sum, grad_out, factor, post, pre, eps, weight_offset,
-                                        gate_rows, dtype, want_out, needs)
-    D = residual.shape[-1]
-    given = (residual, branch, *params)
-    if residual.numel() == 0:
-        return [torch.zeros_like(t) if need and t is not None else None for t, need in zip(given, needs)]
-    grads = [t.new_empty(t.shape) if need and t is not None else None for t, need in zip(given, needs)]
-    ld_sum = ld_out = D
-    if grad_sum is not None:
-        grad_sum, ld_sum = _as_rows(grad_sum, D)
-    if grad_out is not None:
-        grad_out, ld_out = _as_rows(grad_out, D)
-    # of the forward pass's results only whether there was an `out` counts: any address stands for it
-    total, out = (None if branch is None else residual), (stats if want_out else None)
-    packed, keep = _pack_block_norm(residual, branch, total, out, stats, params, factor, post, pre, eps, weight_offset, gate_rows, dtype)
-    want = _nm.BLOCK_NORM_GRADS.pack(ld_sum, ld_out, D, D, _at(grad_sum), _at(grad_out), *[_at(g) for g in grads])
-    lib = _nm.lib()
-    need = lib.nmspmm_block_norm_workspace_bytes(residual.numel() // D, gate_rows, D)
-    workspace = residual.new_empty(need // 4, dtype=torch.float32)
-    _call(lib.nmspmm_block_norm_backward, packed, want, workspace.data_ptr(), need, _stream_of(index))
-    return grads
-
-
-class _BlockNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, residual, branch, gate, scale, post_w, post_b, pre_w, pre_b, conf):
-        factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out = conf
-        params = (gate, scale, post_w, post_b, pre_w, pre_b)
-        total, out, stats = _block_norm_forward(residual, branch, params, *conf, True)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(residual, branch, *params, stats)
-        ctx.conf = conf
-        # without a branch the sum is the residual, as an output of its own: its gradient comes to the same kernel
-        return residual.view_as(residual) if total is None else total, out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_sum, grad_out):
-        residual, branch, *params, stats = ctx.saved_tensors
-        if grad_sum is None and grad_out is None:
-            return (None,) * 9
-        return (*_block_norm_backward(residual, branch, params, stats, grad_sum, grad_out, *ctx.conf, ctx.needs_input_grad[:8]), None)
-
-
-# The same for tracing front ends: one node forward, one backward.  What is not wanted is an empty tensor.
+# For tracing front ends: one node forward, one backward.  What is not wanted is an empty tensor.
 
 @torch.library.custom_op("nmspmm::block_norm", mutates_args=(), device_types="cuda")
 def _block_norm_op(residual: torch.Tensor, branch: Optional[torch.Tensor], gate: Optional[torch.Tensor], scale: Optional[torch.Tensor],
                    post_weight: Optional[torch.Tensor], post_bias: Optional[torch.Tensor], pre_weight: Optional[torch.Tensor],
                    pre_bias: Optional[torch.Tensor], factor: float, post: int, pre: int, eps: float, weight_offset: float,
                    gate_rows: int, dtype: torch.dtype, want_out: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    total, out, stats = _block_norm_forward(residual, branch, (gate, scale, post_weight, post_bias, pre_weight, pre_bias), factor, post,
-                                            pre, eps, weight_offset, gate_rows, dtype, want_out, True)
+    total, out, stats = _binding().block_norm_forward([residual, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias], factor,
+                                                      post, pre, eps, weight_offset, gate_rows, dtype, want_out)
     nothing = lambda: residual.new_empty(0)  # noqa: E731
     return nothing() if total is None else total, nothing() if out is None else out, stats
 
@@ -476,8 +339,8 @@ def _block_norm_backward_op(residual: torch.Tensor, branch: Optional[torch.Tenso
                             grad_sum: Optional[torch.Tensor], grad_out: Optional[torch.Tensor], factor: float, post: int, pre: int,
                             eps: float, weight_offset: float, gate_rows: int, dtype: torch.dtype, want_out: bool,
                             needs: List[bool]) -> List[torch.Tensor]:
-    grads = _block_norm_backward(residual, branch, (gate, scale, post_weight, post_bias, pre_weight, pre_bias), stats, grad_sum, grad_out,
-                                 factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out, needs)
+    grads = _binding().block_norm_backward([residual, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias], stats, grad_sum,
+                                           grad_out, factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out, needs)
     return [residual.new_empty(0) if g is None else g for g in grads]
 
 
@@ -545,50 +408,23 @@ def block_norm(residual, branch=None, *, gate=None, residual_scale=1.0, post=Non
     tensor; gradients repeat bit for bit.  (As with any torch operator, capture a backward pass into a graph only while no eager
     autograd graph over the same leaves is alive.)
     """
-    if not residual.is_cuda or residual.dtype not in _TYPES or residual.dim() < 1:
-        raise ValueError("residual must be a float32, bfloat16 or float16 CUDA tensor")
-    shape, D, device = residual.shape, residual.shape[-1], residual.device
-    if not 0 < D <= 16384:
-        raise ValueError("rows must have 1 to 16384 features, got %d" % D)
-    if dtype is None:
-        dtype = residual.dtype if branch is None else branch.dtype
     if post not in _NORMS or pre not in _NORMS:
         raise ValueError('post and pre are "rms", "layer" or None')
-    if dtype not in _TYPES or residual.dtype not in (dtype, torch.float32):
-        raise ValueError("residual must be float32 or of the type of what the next block takes")
     scale, factor = (residual_scale, 1.0) if isinstance(residual_scale, torch.Tensor) else (None, float(residual_scale))
-    gate_rows = rows = residual.numel() // D
-    if branch is None:
-        if gate is not None or scale is not None or factor != 1.0 or post is not None or pre is None:
-            raise ValueError("without a branch there is a norm before the next block and nothing else")
-    else:
-        if branch.shape != shape or branch.device != device or branch.dtype != dtype:
-            raise ValueError("branch must have residual's shape and device and the type of what the next block takes")
-        if gate is not None:
-            gate, gate_rows = _gate_rows(gate, shape)
-        if scale is not None and scale.shape != (D,):
-            scale = scale.reshape(-1).expand(D)
-    if (post is None and (post_weight is not None or post_bias is not None)) or \
-            (pre is None and (pre_weight is not None or pre_bias is not None)):
-        raise ValueError("a weight or a bias belongs to a norm")
-    params = (gate, scale, post_weight, post_bias, pre_weight, pre_bias)
-    tracked = residual.requires_grad or (branch is not None and branch.requires_grad)
-    for k, p in enumerate(params):
-        if p is not None:
-            if p.device != device or p.dtype not in _TYPES or (k > 0 and p.shape != (D,)):
-                raise ValueError("%s must be a float32, bfloat16 or float16 tensor [%d] on residual's device" % (_PARAMS[k], D))
-            tracked = tracked or p.requires_grad
-    if not eps >= 0.0:
-        raise ValueError("eps must not be negative")
-    conf = (factor, _NORMS[post], _NORMS[pre], eps, weight_offset, max(gate_rows, 1), dtype, pre is not None)
-    if torch.compiler.is_compiling() or type(residual) is not torch.Tensor and type(residual) is not torch.nn.Parameter:
-        total, out, _ = _block_norm_op(residual, branch, *params, *conf)
-        total, out = (None if branch is None else total), (None if pre is None else out)
-    elif tracked and torch.is_grad_enabled():
-        return _BlockNorm.apply(residual, branch, *params, conf)
-    else:
-        total, out, _ = _block_norm_forward(residual, branch, params, *conf, False)
-    return (residual if branch is None else total), out
+    if not torch.compiler.is_compiling() and type(residual) in (torch.Tensor, torch.nn.Parameter):
+        return _binding().block_norm(residual, branch, gate, scale, factor, _NORMS[post], post_weight, post_bias, _NORMS[pre], pre_weight,
+                                     pre_bias, eps, weight_offset, dtype)
+    D = residual.shape[-1]
+    if dtype is None:
+        dtype = residual.dtype if branch is None else branch.dtype
+    gate_rows = residual.numel() // D
+    if gate is not None:
+        gate, gate_rows = _gate_rows(gate, residual.shape)
+    if scale is not None and scale.shape != (D,):
+        scale = scale.reshape(-1).expand(D)
+    total, out, _ = _block_norm_op(residual, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias, factor, _NORMS[post],
+                                   _NORMS[pre], eps, weight_offset, max(gate_rows, 1), dtype, pre is not None)
+    return (residual if branch is None else total), (None if pre is None else out)
 
 
 class NMBlockStack(torch.nn.Module):

@@ -336,10 +336,12 @@ def test_rows_that_are_constant_zero_large_or_not_finite():
 def test_sum_may_overwrite_the_residual_and_out_the_branch():
     t, conf, dt = make(11, (40, 512), "bf16", "same", "fp32", gate="sample")
     want = call(t, conf, dt)
-    m = op()
     params = tuple(t[k] for k in ("gate", "scale", "post_weight", "post_bias", "pre_weight", "pre_bias"))
     r, y = t["residual"].clone(), t["branch"].clone()
-    packed, _ = m._pack_block_norm(r, y, r, y, None, params, 1.0, 1, 1, EPS, 0.0, 1, dt)
+    code = {torch.float32: nmspmm.F32, torch.bfloat16: nmspmm.BF16}
+    packed = nmspmm.BLOCK_NORM.pack(40, 1, 512, 512, 512, 512, r.data_ptr(), y.data_ptr(), r.data_ptr(), y.data_ptr(), 0,
+                                    *[0 if p is None else p.data_ptr() for p in params], *[0 if p is None else code[p.dtype] for p in params],
+                                    512, code[dt], code[r.dtype], 1, 1, 1.0, EPS, 0.0)
     assert nmspmm.lib().nmspmm_block_norm_forward(packed, torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(r, want[0]) and torch.equal(y, want[1])
 
@@ -457,6 +459,58 @@ def test_refusals():
     d, = torch.autograd.grad(f(x, r)[1].sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(d.sum(), x)
+
+
+def test_operators_refuse_what_does_not_fit():
+    """The traced operators take each other's results by hand too: sizes are checked there as well."""
+    r, w = torch.randn((4, 64), device="cuda"), torch.ones(64, device="cuda")
+    ops = torch.ops.nmspmm
+    conf = (1.0, 1, 1, EPS, 0.0, 4, torch.float32, True)
+    total, out, stats = ops.block_norm(r, r, w, None, w, None, w, None, *conf)
+    given = (r, r, w, None, w, None, w, None)
+    needs = [t is not None for t in given]
+    grads = ops.block_norm_backward(*given, stats, total, out, *conf, needs)
+    assert [g.shape == t.shape if t is not None else g.numel() == 0 for g, t in zip(grads, given)] == [True] * 8
+    for bad in (stats[:3], stats.double(), stats.cpu()):
+        with pytest.raises((ValueError, NotImplementedError)):
+            ops.block_norm_backward(*given, bad, total, out, *conf, needs)
+    for d in (total[:3], total.bfloat16()):
+        with pytest.raises(ValueError):
+            ops.block_norm_backward(*given, stats, d, None, *conf, needs)
+        with pytest.raises(ValueError):
+            ops.block_norm_backward(*given, stats, None, d, *conf, needs)
+    for kw in (dict(gate=w[:63]), dict(gate_rows=3), dict(post=3), dict(dtype=torch.float64)):
+        a, c = list(given), list(conf)
+        if "gate" in kw:
+            a[2] = kw["gate"]
+        else:
+            c[dict(gate_rows=5, post=1, dtype=6)[next(iter(kw))]] = next(iter(kw.values()))
+        with pytest.raises(ValueError):
+            ops.block_norm(*a, *c)
+
+
+def test_hooks_retained_graphs_and_checkpoints():
+    """What autograd does around a node: saved tensors go through hooks, a graph is walked twice, a part is run again."""
+    t, conf, dt = make(23, (6, 96), "bf16", "fp32", "fp32", gate="sample")
+    leaves = [v.requires_grad_(True) for v in t.values() if v is not None]
+
+    def run():
+        total, out = call(t, conf, dt)
+        return total.sum() + out.float().square().sum()
+
+    want = torch.autograd.grad(run(), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        loss = run()
+    for _ in range(2):
+        for a, b in zip(torch.autograd.grad(loss, leaves, retain_graph=True), want):
+            assert torch.equal(a, b)
+    again = torch.utils.checkpoint.checkpoint(run, use_reentrant=False)
+    for a, b in zip(torch.autograd.grad(again, leaves), want):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(again, leaves)      # freed
+    for k, leaf in enumerate(leaves):            # each gradient alone, as when the others are frozen
+        assert torch.equal(torch.autograd.grad(run(), leaf)[0], want[k])
 
 
 @pytest.mark.parametrize("norm", ["rms", "layer"])

@@ -417,3 +417,25 @@ def test_refusals():
         op().NMQuantOperand.from_codes(cuda(codes), cuda(scale), None, 512, n=1, m=2)     # no rows
     with pytest.raises(ValueError):
         op().NMQuantOperand.quantize(torch.randn((256, 64), device="cuda"), torch.zeros((256, 2), dtype=torch.int32, device="cuda"), 256)
+
+
+def test_the_operator_refuses_buffers_that_are_not_the_operands():
+    codes, scale, zero, rows, _ = make(2, 256, 64, 2, 4)
+    o = op().NMQuantOperand.from_codes(cuda(codes), cuda(scale), cuda(zero), 256, 2, 4, cuda(rows))
+    x = torch.randn((3, 256), device="cuda")
+    good = [x, o.codes, o.scales, o.row_offsets, None, 256, 64, 2, 4, 128]
+    f = torch.ops.nmspmm.quant_linear
+    want = f(*good)
+    assert torch.equal(f(*good[:4], torch.zeros(64, device="cuda", dtype=torch.bfloat16), *good[5:]), want)
+    for at, bad in ((1, o.codes[:-1]), (1, o.codes[::2]), (2, o.scales[:-1]), (3, o.row_offsets[:-1]), (3, None), (4, x[0, :63]),
+                    (4, x[:, :64]), (6, 96), (6, 0), (6, 1 << 40), (7, 3), (8, 5), (8, 1), (9, 48), (9, 0)):
+        args = list(good)
+        args[at] = bad
+        with pytest.raises(ValueError):
+            f(*args)
+
+
+def test_too_many_rows_are_refused():
+    o = op().NMQuantLinear.from_codes(torch.zeros((1, 1), dtype=torch.uint8, device="cuda"), torch.ones((1, 1), device="cuda"), None, 1)
+    with pytest.raises(ValueError):
+        o(torch.zeros(((1 << 24) + 1, 1), dtype=torch.float16, device="cuda"))
