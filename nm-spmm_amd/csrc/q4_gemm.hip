@@ -468,8 +468,8 @@ bool q4_densifies(const Q4Shape& p, int M) { return p.m > 1 && M > 16; }
 
 size_t q4_workspace_bytes(const Q4Shape& p, int M, ElementType type)
 {
-    // (whether 9 to 16 rows of 16-bit elements are aligned is not known here)
-    return gemm_space(p, M, type, q4_densifies(p, M), M > (type == kF32 || p.m > 1 ? 16 : 8)).bytes;
+    // (how 9 to 16 rows are aligned and grouped is not known here)
+    return gemm_space(p, M, type, q4_densifies(p, M), M > (p.m > 1 ? 16 : 8)).bytes;
 }
 
 hipError_t launch_q4_densify(const Q4LinearArgs& a, uint32_t* out)

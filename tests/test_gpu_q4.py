@@ -128,6 +128,37 @@ def test_rows_of_x_with_strides(dtype, layout, M, K, N, n, m):
     run(M, M, K, N, dtype, n, m, layout=layout)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,m", [(1, 2), (2, 4), (4, 8), (8, 16)])
+@pytest.mark.parametrize("M,K,N,group", [(5, 272, 96, 32), (8, 2064, 32, 128), (9, 16, 32, 64), (13, 784, 64, 128), (16, 1536, 64, 32),
+                                         (11, 528, 8256, 64), (7, 528, 8256, 32)])
+def test_aligned_rows_of_a_half_kept_operand(dtype, n, m, M, K, N, group):
+    """Rows that are read whole and gathered afterwards: what lies behind them and what they hold in places that are not
+    kept does not count, and the result is that of rows which cannot be read so."""
+    layer, x, y = run(M + K, M, K, N, dtype, n, m, group)
+    wide = torch.full((M, K + 8), float("nan"), dtype=x.dtype, device="cuda")
+    wide[:, :K] = x
+    assert torch.equal(layer(wide[:, :K]), y)
+    odd = torch.full((M, K + 5), float("nan"), dtype=x.dtype, device="cuda")[:, 3:3 + K]
+    odd.copy_(x)
+    # the same products in the same order, whichever way the elements came
+    assert torch.equal(layer(odd), y)
+    first = layer.row_offsets.view(N // 32, -1)[0, :1].item()       # in the first 32 columns not kept: the first window's first other row
+    lost = 1 if first == 0 else 0
+    if n == 1:
+        wide[:, lost] = float("inf")
+        y2 = layer(wide[:, :K])
+        assert torch.equal(y2[:, :32], y[:, :32])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,n,m", [(1, 1, 1), (4, 1, 1), (7, 1, 1), (13, 1, 1), (16, 1, 1), (6, 2, 8), (16, 2, 8), (14, 2, 4)])
+def test_wide_operands(dtype, group, M, n, m):
+    """Enough columns for every compute unit twice over."""
+    run(M + group, M, 416, 8224, dtype, n, m, group)
+
+
 def test_leading_dimensions_and_empty_batches():
     made = make(3, 256, 64)
     layer = layer_of(made, 256)
