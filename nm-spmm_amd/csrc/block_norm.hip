@@ -274,6 +274,8 @@ private:
 };
 
 // ---- forward ------------------------------------------------------------------------------------------
+// 4096 rows of 8192 bf16: 57.5 us (268 MB, 4.7 TB/s, what a copy reaches); 1071 rows of 2049 fp32, whose accesses are not aligned: 22.5
+// (44 MB, 2.0 TB/s); one row of 4096: 4.5, launch and two sums over 512 threads.
 
 template <ElementType T, ElementType R, bool WIDE, int NV, int THREADS, bool BIAS>
 __global__ void __launch_bounds__(THREADS)
@@ -377,6 +379,8 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
 }
 
 // ---- backward -----------------------------------------------------------------------------------------
+// 4096 rows of 4096 bf16, all six parameters: 49 us (201 MB, 4.1 TB/s) and 6.4 to add the walkers' sums up; 1505 rows of 1536 fp32:
+// 18.5 (55 MB, 3.0 TB/s) and 4.8.
 
 template <ElementType T, ElementType R, bool WIDE, int NV, int THREADS, bool BIAS>
 __global__ void __launch_bounds__(THREADS)

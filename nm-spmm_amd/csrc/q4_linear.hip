@@ -40,6 +40,9 @@ __device__ inline __amdgpu_buffer_rsrc_t window(const void* base, size_t bytes)
 // A workgroup takes NC 16-column tiles and at most RT row tiles; its waves take the blocks of 128 kept rows in turn
 // and add up their sums in LDS at the end, in wave order.  A block costs about 60 vector instructions a tile, which is what bounds
 // the kernel beside the launch: addresses are scalars, ends are left to the descriptors' bounds, groups are unrolled.
+// Measured: one row, 4096 x 4096 in fp32 4.0 us (9 MB; the launch alone is over 2); 8192 x 8192 2:8 4.2; 8 rows of bf16, 11008 x 4096 9.8
+// (24 MB, 2.4 TB/s: one workgroup of 16 waves per compute unit, a matrix instruction for half a tile of rows); 13 rows,
+// 4096 x 14336 2:4 11.2 (17 MB).
 // MX: rows of x the instance has registers for; UNITS: scaled groups in a block.
 // What an instance needs registers for decides how many waves it runs with (fp32, 8 rows, 4096 x 4096 in groups of 32: 11.9 us with
 // sixteen waves, which spill, 9.4 with eight; 13 rows of bf16, 4096 x 14336: 23.5 and 19.0).
