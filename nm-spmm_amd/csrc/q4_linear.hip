@@ -42,25 +42,31 @@ __device__ inline __amdgpu_buffer_rsrc_t window(const void* base, size_t bytes)
 // the kernel beside the launch: addresses are scalars, ends are left to the descriptors' bounds, groups are unrolled.
 // Measured: one row, 4096 x 4096 in fp32 4.0 us (9 MB; the launch alone is over 2); 8192 x 8192 2:8 4.2; 8 rows of bf16, 11008 x 4096 9.8
 // (24 MB, 2.4 TB/s: one workgroup of 16 waves per compute unit, a matrix instruction for half a tile of rows); 13 rows,
-// 4096 x 14336 2:4 11.2 (17 MB).
+// 4096 x 14336 2:4 8.4 (17 MB).
 // MX: rows of x the instance has registers for; UNITS: scaled groups in a block.
-// What an instance needs registers for decides how many waves it runs with (fp32, 8 rows, 4096 x 4096 in groups of 32: 11.9 us with
-// sixteen waves, which spill, 9.4 with eight; 13 rows of bf16, 4096 x 14336: 23.5 and 19.0).
-constexpr int most_waves(int RT, int NC, int MX, int UNITS)
+// What an instance needs registers for decides how many waves it runs with (us with sixteen waves, which spill, and eight: 13 rows of
+// bf16, 4096 x 14336 in groups of 32 23.5 and 19.0; fp32, 8 rows, 2:4 in groups of 32 36.6 and 18.2).
+constexpr int most_waves(Source SRC, int RT, int NC, int MX, int UNITS)
 {
-    return MX > 8 || (RT > 1 && MX == 1) || (UNITS == 4 && (RT > 1 || (NC == 2 && MX != 4))) ? kMaxWaves / 2 : kMaxWaves;
+    return (MX > 8 && !(SRC == kSpanned && NC * UNITS < 8)) || (RT > 1 && MX == 1) ||
+                   (UNITS == 4 && (RT > 1 || (NC == 2 && MX != 4))) || (UNITS == 2 && RT > 1 && SRC == kGathered)
+               ? kMaxWaves / 2
+               : kMaxWaves;
 }
 
-// Blocks under way at a time.
+// Blocks under way at a time.  Many rows take many registers: there more waves hide more than more loads of one (13 rows, 4096 x 14336 2:4
+// 11.2 us with two blocks and 180 registers, 8.4 with one and 92; 8 rows of fp32 14.8 and 12.7).  Gathered elements need two.
 constexpr int depth_of(Source src, int RT, int NC, int MX, int UNITS)
 {
+    if ((src == kSpanned || src == kStaged) && MX >= 8)
+        return 1;
     if (src == kDirect)
         return RT == 1 && NC == 1 && UNITS < 4 ? 3 : 2;
     return MX == 1 ? (NC == 1 ? 4 : UNITS < 4 ? 3 : 2) : MX == 4 && NC == 1 ? 3 : 2;
 }
 
 template <ElementType T, Source SRC, int RT, int NC, int MX, int UNITS>
-__global__ void __launch_bounds__(most_waves(RT, NC, MX, UNITS) * 64)
+__global__ void __launch_bounds__(most_waves(SRC, RT, NC, MX, UNITS) * 64)
 q4_rows_product_kernel(const void* __restrict__ x_, size_t ldx, const uint32_t* __restrict__ codes, Q4Meta meta,
                        const uint8_t* __restrict__ rows, const float* __restrict__ bias, void* __restrict__ y, size_t ldy, int M,
                        Q4Shape p, bool pairs)
@@ -312,8 +318,8 @@ hipError_t launch_rows(const Q4LinearArgs& a, bool pairs)
     // one workgroup to a compute unit: sixteen waves each; more workgroups than that: eight (measured, us with 8 / 16 waves:
     // 4096 x 14336 dense 8.7 / 9.3, 2:4 5.7 / 7.0 at one row; 8192 x 8192 9.9 / 8.4, 11008 x 4096 9.3 / 8.0)
     int most = a.p.tiles / NC > machine().cus ? kMaxWaves / 2 : kMaxWaves;
-    if (most > most_waves(RT, NC, MX, UNITS))
-        most = most_waves(RT, NC, MX, UNITS);
+    if (most > most_waves(SRC, RT, NC, MX, UNITS))
+        most = most_waves(SRC, RT, NC, MX, UNITS);
     const size_t staged = SRC == kDirect ? 0 : (size_t)MX * (T == kF32 ? 3 : 1) * (SRC == kSpanned ? kSpanPitch : kRowPitch) * 2;
     const size_t sums = (size_t)Chunk * NC * 16 * sizeof(float);
     const size_t each = staged > sums ? staged : sums;
@@ -339,10 +345,9 @@ bool pair_columns(const Q4LinearArgs& a) { return a.p.tiles >= 2 * machine().cus
 template <ElementType T, Source SRC, int RT, int MX, int UNITS>
 hipError_t launch_columns(const Q4LinearArgs& a, bool pairs)
 {
-    // fp32 rows of small groups hold too much for two tiles (4096 x 14336, us with two / one: 8 rows, groups of 32: 82 / 32, of 64: 35 /
-    // 20); nine or more of them are gathered here or have groups of 128
-    constexpr bool both = !(T == kF32 && ((MX == 8 && UNITS > 1) || (MX == 16 && UNITS > (SRC == kGathered ? 2 : 1)))) &&
-                          !(SRC == kSpanned && MX == 8);
+    // nine and more fp32 rows of small groups hold too much for two tiles (13 rows, 4096 x 14336, groups of 32: 78 us; the dense ones
+    // of them are not taken here at all)
+    constexpr bool both = !(T == kF32 && MX == 16 && UNITS > (SRC == kGathered ? 2 : 1));
     if constexpr (both)
         if (pair_columns(a))
             return launch_rows<T, SRC, RT, 2, MX, UNITS>(a, pairs);
@@ -369,9 +374,10 @@ hipError_t launch_source(const Q4LinearArgs& a, bool pairs)
             if (a.M <= 4)
                 return launch_units<T, SRC, 1, 4>(a, pairs);
         }
-        if (a.M <= 8)
-            return launch_units<T, SRC, T == kF32 ? 2 : 1, 8>(a, pairs);
-        return launch_units<T, SRC, T == kF32 ? 4 : 1, 16>(a, pairs);
+        if constexpr (T != kF32 && SRC == kStaged)      // (few_rows)
+            return launch_units<T, SRC, 1, 8>(a, pairs);
+        else
+            return a.M <= 8 ? launch_units<T, SRC, T == kF32 ? 2 : 1, 8>(a, pairs) : launch_units<T, SRC, T == kF32 ? 4 : 1, 16>(a, pairs);
     }
 }
 
@@ -382,17 +388,16 @@ bool direct(const Q4LinearArgs& a, ElementType type)
 }
 
 // All elements that a block spans are read, in whole 16-byte pieces, where gathering would be what bounds the kernel (us, gathered
-// in memory / in LDS: 4096 x 14336 2:4 at 13 rows 13.7 / 11.2, at 8 rows, two column tiles, 8.0 / 8.8; 4096 x 4096 at 8 rows 4.8 / 4.4,
-// at 4 rows 3.7 / 4.1).
+// in memory / in LDS: 4096 x 14336 2:4 at 13 rows 13.7 / 8.4, at 8 rows 8.0 / 6.8; 4096 x 4096 at 8 rows 4.8 / 4.5, at 4 rows 3.7 / 4.1).
 bool spanned(const Q4LinearArgs& a)
 {
-    return (a.M > 8 || (a.M > 4 && !pair_columns(a))) && a.p.m == 2 * a.p.n && a.p.K % 8 == 0 && a.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15u) == 0;
+    return a.M > 4 && a.p.m == 2 * a.p.n && a.p.K % 8 == 0 && a.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15u) == 0;
 }
 
 // Whether the kernel above takes the rows.  Measured against the other one (q4_gemm.hip), us at 4096 x 4096: as they lie, 16 / 32
 // rows 6.4 / 10.1 against 12 / 14.3 (11008 x 4096: 14 / 23.4 against 17.5 with 32); fp32, 8 / 16 rows 6.9 / 12.0 against 12.3 / 13.9;
 // 16-bit rows that are not aligned, 16 of them 27.9 against 12; at 4096 x 14336 fp32, 13 against 17 rows, groups of 128 / 64 / 32
-// 23.6 / 29.8 / 49.4 against 24.0 / 24.6 / 32.4.
+// 23.2 / 29.8 / 49.4 against 24.0 / 24.6 / 32.4.
 bool few_rows(const Q4LinearArgs& a, ElementType type)
 {
     if (direct(a, type))
