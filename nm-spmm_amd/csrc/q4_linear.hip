@@ -19,7 +19,7 @@ namespace {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kMaxWaves = 16;
-constexpr size_t kMostLds = 131072;
+constexpr size_t kMostLds = 163840;     // all of a compute unit's: sixteen waves of sixteen half-kept rows take 135 KB
 constexpr int kRowPitch = 136;      // 16-bit elements between staged rows: 128 and 16 bytes, so that the sixteen
                                     // rows of a 128-bit LDS read start in different banks
 
