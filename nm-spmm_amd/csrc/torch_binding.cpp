@@ -52,12 +52,21 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 
 const void* at_of(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
+// What lies in memory is what t stands for, and no tangent of forward-mode differentiation is lost.
+Tensor plain(const Tensor& t)
+{
+    if (!t.defined())
+        return t;
+    require(!t._fw_grad(0).defined(), "there is no forward-mode derivative");
+    return t.is_neg() ? t.resolve_neg() : t;
+}
+
 // ---- operands in 4 bits --------------------------------------------------------------------------------
 
 Tensor quant_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& row_offsets, const OptTensor& bias,
                     int64_t K, int64_t N, int64_t n, int64_t m, int64_t group)
 {
-    require(K >= 1 && N >= 1 && K <= INT_MAX && N <= INT_MAX && n >= 1 && m >= n && m <= 64 && group >= 1 && group <= 128,
+    require(K >= 1 && N >= 1 && K <= INT_MAX && N <= INT_MAX && n >= 1 && m >= n && m <= INT_MAX && group >= 1 && group <= 128,
             "no operand of ", K, " x ", N, " with pattern ", n, ":", m, " and groups of ", group);
     const int type = type_of(x.scalar_type());
     require(x.is_cuda() && type >= 0 && x.dim() >= 1 && x.size(-1) == K,
@@ -72,7 +81,7 @@ Tensor quant_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, 
                       "codes, scales and row offsets must be those of an operand of ", K, " x ", N, ", on the device of x");
     if (plus.defined()) {
         require(plus.device() == x.device() && plus.dim() == 1 && plus.size(0) == N, "bias must have ", N, " elements on the device of x");
-        plus = plus.to(at::kFloat).contiguous();
+        plus = plain(plus).to(at::kFloat).contiguous();
     }
     const c10::DeviceGuard guard(x.device());
     auto shape = x.sizes().vec();
@@ -81,10 +90,10 @@ Tensor quant_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, 
     const int64_t M = y.numel() / N;
     if (M == 0)
         return y;
-    Tensor from = x;
+    Tensor from = plain(x);
     int64_t ldx = K;
-    if (!x.is_contiguous()) {
-        from = x.reshape({M, K});
+    if (!from.is_contiguous()) {
+        from = from.reshape({M, K});
         if (M > 1)
             ldx = from.stride(0);
         if ((K > 1 && from.stride(1) != 1) || ldx < K || ldx > (1 << 24)) {
@@ -133,8 +142,9 @@ using Given = std::array<Tensor, kGiven>;
 const char* const kNames[kGiven] = {"residual", "branch", "gate", "residual_scale", "post_weight", "post_bias", "pre_weight", "pre_bias"};
 
 // t where its leading dimensions can be walked as rows, else a copy; and the elements between its rows.
-std::pair<Tensor, int64_t> as_rows(const Tensor& t, int64_t D)
+std::pair<Tensor, int64_t> as_rows(const Tensor& given, int64_t D)
 {
+    const Tensor t = plain(given);
     if (!t.defined() || t.is_contiguous())
         return {t, D};
     Tensor rows = t.reshape({-1, D});
@@ -196,7 +206,7 @@ nmspmm_block_norm block_of(const Given& g, const Conf& c, const Tensor& total, c
         const Tensor& t = g[i + 2];
         if (!t.defined())
             continue;
-        const Tensor whole = t.contiguous();
+        const Tensor whole = plain(t).contiguous();
         *data[i] = whole.const_data_ptr();
         *type[i] = type_of(whole.scalar_type());
         if (!whole.is_same(t))

@@ -489,6 +489,27 @@ def test_operators_refuse_what_does_not_fit():
             ops.block_norm(*a, *c)
 
 
+def test_negated_views_and_tangents():
+    """A view whose memory holds the negated values counts as what it stands for; forward-mode derivatives are refused."""
+    z = torch.randn((5, 64), dtype=torch.complex64, device="cuda")
+    r, w = z.conj().imag, torch.randn((64,), dtype=torch.complex64, device="cuda").conj().imag
+    assert r.is_neg() and w.is_neg()
+    got = op().block_norm(r, r, gate=w, post="rms", post_weight=w, pre_weight=w)
+    plain, pw = -z.imag, w.resolve_neg()
+    for a, b in zip(got, op().block_norm(plain, plain, gate=pw, post="rms", post_weight=pw, pre_weight=pw)):
+        assert torch.equal(a, b)
+    x = plain.clone().requires_grad_(True)
+    total, out = op().block_norm(x, plain, pre_weight=pw)
+    d1, = torch.autograd.grad((total, out), x, (r, r), retain_graph=True)
+    d2, = torch.autograd.grad((total, out), x, (plain, plain))
+    assert torch.equal(d1, d2)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(plain.contiguous(), torch.ones_like(plain))
+        for args in ((dual,), (plain, dual)):
+            with pytest.raises((ValueError, RuntimeError)):
+                op().block_norm(*args)
+
+
 def test_hooks_retained_graphs_and_checkpoints():
     """What autograd does around a node: saved tensors go through hooks, a graph is walked twice, a part is run again."""
     t, conf, dt = make(23, (6, 96), "bf16", "fp32", "fp32", gate="sample")

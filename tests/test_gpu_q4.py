@@ -470,3 +470,20 @@ def test_too_many_rows_are_refused():
     o = op().NMQuantLinear.from_codes(torch.zeros((1, 1), dtype=torch.uint8, device="cuda"), torch.ones((1, 1), device="cuda"), None, 1)
     with pytest.raises(ValueError):
         o(torch.zeros(((1 << 24) + 1, 1), dtype=torch.float16, device="cuda"))
+
+
+def test_negated_views_and_tangents():
+    layer = layer_of(make(4, 256, 64), 256)
+    z = torch.randn((3, 256), dtype=torch.complex64, device="cuda")
+    x = z.conj().imag
+    assert x.is_neg() and torch.equal(layer(x), layer(-z.imag))
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises((ValueError, RuntimeError)):
+            layer(torch.autograd.forward_ad.make_dual(z.real.contiguous(), z.real.contiguous()))
+
+
+def test_a_dense_operand_may_be_named_by_any_n_and_m():
+    codes, scale, zero, _, _ = make(6, 300, 40)
+    a, b = (op().NMQuantLinear.from_codes(cuda(codes), cuda(scale), cuda(zero), 300, n, n) for n in (1, 100))
+    x = torch.randn((2, 300), device="cuda")
+    assert torch.equal(a(x), b(x))
