@@ -317,9 +317,14 @@ def q4_operand(codes, meta, row_offsets, K, N, n=1, m=1, group=128, bias=None):
     return Q4Operand(*at, K, N, n, m, group)
 
 
+def q4_kept_rows(K, n, m):
+    """Rows of the compressed operand: all K of a dense one, whatever n = m is."""
+    return K if n == m else K // max(m, 1) * n
+
+
 def q4_quantize_device(dBT, dDT, op, flags=0):
     """float32[W][N] (and int32[W][N/32] when n < m) -> the operand's buffers."""
-    W = op.K // max(op.m, 1) * op.n
+    W = q4_kept_rows(op.K, op.n, op.m)
     _need("q4_quantize_device", dBT=(dBT, W * op.N), dDT=(dDT, W * (op.N // 32)))
     _check("nmspmm_q4_quantize_device",
            lib().nmspmm_q4_quantize_device(_ptr(dBT), _ptr(dDT), ctypes.byref(op), flags, _stream()))
@@ -327,7 +332,7 @@ def q4_quantize_device(dBT, dDT, op, flags=0):
 
 def q4_pack_device(d_codes, d_scales, d_zeros, dDT, op):
     """uint8[W][N] codes, float32[groups][N] scales, uint8[groups][N] zero points (or None) -> the operand's buffers."""
-    W = op.K // max(op.m, 1) * op.n
+    W = q4_kept_rows(op.K, op.n, op.m)
     groups = -(-W // max(op.group, 1))
     _need("q4_pack_device", d_codes=(d_codes, W * op.N), d_scales=(d_scales, groups * op.N), d_zeros=(d_zeros, groups * op.N),
           dDT=(dDT, W * (op.N // 32)))

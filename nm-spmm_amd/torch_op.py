@@ -159,6 +159,11 @@ def _guard(tensor):
     return torch.cuda.device(tensor.device)
 
 
+def _floats(t):
+    """float32, contiguous, and in memory what it stands for (a view of a complex tensor's conjugate may not be)."""
+    return t.to(torch.float32).contiguous().resolve_neg()
+
+
 class NMQuantOperand:
     """An operand B [K, N] in 4 bits (nmspmm.h: nmspmm_q4_operand): codes with a scale and a zero point
     per group of kept rows and column; n == m == 1 is a dense operand."""
@@ -192,19 +197,20 @@ class NMQuantOperand:
     def quantize(cls, values, rows, K, n=1, m=1, group=128, asymmetric=False):
         """From float values [K * n / m, N] and their window-local row numbers [K * n / m, N / 32] (None when n == m)."""
         if values.dim() != 2 or not values.is_cuda or not values.is_floating_point() or n < 1 or m < n or \
-                values.shape[0] != K // m * n:
+                values.shape[0] != _nm.q4_kept_rows(K, n, m):
             raise ValueError("values must be a 2-D floating CUDA tensor of K * n / m rows")
         operand = cls(K, values.shape[1], n, m, group, values.device)
         rows = operand._rows(rows, values)
         with _guard(values):
-            _nm.q4_quantize_device(values.to(torch.float32).contiguous(), rows, operand._struct(),
+            _nm.q4_quantize_device(_floats(values), rows, operand._struct(),
                                    _nm.Q4_ASYMMETRIC if asymmetric else 0)
         return operand
 
     @classmethod
     def from_codes(cls, codes, scale, zero, K, n=1, m=1, rows=None, group=128):
         """From codes 0..15 [W, N] (W = K * n / m), scale and zero [ceil(W / group), N]; zero None stands for 8."""
-        if codes.dim() != 2 or not codes.is_cuda or codes.dtype != torch.uint8 or n < 1 or m < n or codes.shape[0] != K // m * n:
+        if codes.dim() != 2 or not codes.is_cuda or codes.dtype != torch.uint8 or n < 1 or m < n or \
+                codes.shape[0] != _nm.q4_kept_rows(K, n, m):
             raise ValueError("codes must be a 2-D uint8 CUDA tensor of K * n / m rows")
         operand = cls(K, codes.shape[1], n, m, group, codes.device)
         per_group = (-(-codes.shape[0] // group), codes.shape[1])
@@ -214,7 +220,7 @@ class NMQuantOperand:
             raise ValueError("zero must be a tensor %s of whole numbers 0..15 on the device of the codes" % (per_group,))
         rows = operand._rows(rows, codes)
         with _guard(codes):
-            _nm.q4_pack_device(codes.contiguous(), scale.to(torch.float32).contiguous(),
+            _nm.q4_pack_device(codes.contiguous(), _floats(scale),
                                None if zero is None else zero.to(torch.uint8).contiguous(), rows, operand._struct())
         return operand
 
@@ -255,7 +261,7 @@ class NMQuantLinear(torch.nn.Module):
         N, K = weight.shape
         if n != m and (n < 1 or m < n or K % m != 0 or N % 32 != 0 or m not in (4, 8, 16, 32)):
             raise ValueError("pattern %d:%d needs m of 4, 8, 16 or 32, in_features a multiple of it and out_features of 32" % (n, m))
-        values, rows = weight.detach().t().to(torch.float32).contiguous(), None
+        values, rows = _floats(weight.detach().t()), None
         if n != m:
             dense, W = values, K // m * n
             values = torch.empty((W, N), dtype=torch.float32, device=weight.device)
@@ -280,7 +286,7 @@ class NMQuantLinear(torch.nn.Module):
         self.register_buffer("codes", operand.codes)
         self.register_buffer("scales", operand.scales)
         self.register_buffer("row_offsets", operand.row_offsets)
-        self.register_buffer("bias", None if bias is None else bias.detach().to(torch.float32).contiguous())
+        self.register_buffer("bias", None if bias is None else _floats(bias.detach()))
 
     def _operand(self):
         b = self._buffers

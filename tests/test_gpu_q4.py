@@ -477,6 +477,8 @@ def test_negated_views_and_tangents():
     z = torch.randn((3, 256), dtype=torch.complex64, device="cuda")
     x = z.conj().imag
     assert x.is_neg() and torch.equal(layer(x), layer(-z.imag))
+    w = torch.randn((32, 64), dtype=torch.complex64, device="cuda").conj().imag
+    assert torch.equal(op().NMQuantLinear(w).dense_weight(), op().NMQuantLinear(w.resolve_neg()).dense_weight())
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises((ValueError, RuntimeError)):
             layer(torch.autograd.forward_ad.make_dual(z.real.contiguous(), z.real.contiguous()))
@@ -484,6 +486,12 @@ def test_negated_views_and_tangents():
 
 def test_a_dense_operand_may_be_named_by_any_n_and_m():
     codes, scale, zero, _, _ = make(6, 300, 40)
-    a, b = (op().NMQuantLinear.from_codes(cuda(codes), cuda(scale), cuda(zero), 300, n, n) for n in (1, 100))
+    a, b, c = (op().NMQuantLinear.from_codes(cuda(codes), cuda(scale), cuda(zero), 300, n, n) for n in (1, 100, 7))
     x = torch.randn((2, 300), device="cuda")
-    assert torch.equal(a(x), b(x))
+    assert torch.equal(a(x), b(x)) and torch.equal(a(x), c(x))
+    v = torch.randn((300, 40), device="cuda")
+    assert torch.equal(op().NMQuantOperand.quantize(v, None, 300).dense(), op().NMQuantOperand.quantize(v, None, 300, 7, 7).dense())
+    with pytest.raises(ValueError):     # all rows of a dense operand, not the 294 of whole windows
+        op().NMQuantOperand.quantize(v[:294], None, 300, 7, 7)
+    with pytest.raises(ValueError):
+        op().NMQuantOperand.from_codes(cuda(codes)[:294], cuda(scale), cuda(zero), 300, 7, 7)

@@ -83,3 +83,7 @@ def test_binding_checks_what_the_pointers_hold():
         nmspmm.q4_linear(op, torch.zeros(256), torch.zeros(63), 1, nmspmm.F32)
     with pytest.raises(ValueError):
         nmspmm.q4_expand_device(op, torch.zeros(16))
+
+
+def test_kept_rows():
+    assert [nmspmm.q4_kept_rows(*a) for a in ((300, 1, 1), (300, 7, 7), (300, 2, 4), (64, 1, 8))] == [300, 300, 150, 8]
