@@ -80,7 +80,7 @@ size_t nmspmm_q4_workspace_bytes(int M, int K, int N, int n, int m, int type)
 {
     Q4Shape p;
     if (M <= 0 || M > (1 << 24) || (type != NMSPMM_F32 && type != NMSPMM_BF16 && type != NMSPMM_F16) ||
-        q4_shape(K, N, n, m, 128, &p) != NMSPMM_OK)
+        q4_shape(K, N, n, m, 32, &p) != NMSPMM_OK)     // (the group is not known here: groups of 32 take no less than larger ones)
         return 0;
     return q4_workspace_bytes(p, M, (ElementType)type);
 }

@@ -606,7 +606,8 @@ hipError_t launch_q4_expand(const uint32_t* codes, const uint32_t* meta, const u
 // The workspace holds what q4_workspace_bytes says; 0 bytes: it may be nullptr.
 size_t q4_workspace_bytes(const Q4Shape& p, int M, ElementType type);
 hipError_t launch_q4_linear(const Q4LinearArgs& a, ElementType type, void* workspace);
-bool q4_densifies(const Q4Shape& p, int M);
+int q4_gathered_rows(const Q4Shape& p, ElementType type);
+bool q4_densifies(const Q4Shape& p, int M, ElementType type);
 hipError_t launch_q4_densify(const Q4LinearArgs& a, uint32_t* out);
 hipError_t launch_q4_gemm(const Q4LinearArgs& a, ElementType type, bool densified, void* workspace);
 

@@ -40,6 +40,24 @@ __device__ inline u32x4 widened(uint32_t w, uint32_t one)
     return u32x4{(w & mask) | one, ((w >> 4) & mask) | one, ((w >> 8) & mask) | one, (__builtin_amdgcn_alignbit(w, w, 12) & mask) | one};
 }
 
+// Eight 8-bit floats that stand for code - zero times 2^-9 -> eight operand elements code - zero (exact).
+template <ElementType T>
+__device__ inline u32x4 from_bytes(uint32_t low, uint32_t high)
+{
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const float unit = 512.0f;
+    if (T == kF16)
+        return u32x4{__builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(low, unit, false)),
+                     __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(low, unit, true)),
+                     __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(high, unit, false)),
+                     __builtin_bit_cast(uint32_t, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(high, unit, true))};
+    return u32x4{__builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(low, unit, false)),
+                 __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(low, unit, true)),
+                 __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, unit, false)),
+                 __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, unit, true))};
+}
+
 template <ElementType T>
 __device__ inline void store_result(void* y, size_t at, float v)
 {

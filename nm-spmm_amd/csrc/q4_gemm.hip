@@ -6,6 +6,7 @@
 // elements, two buffers, 16-byte pieces swapped by row so that the sixteen rows of a read lie in different
 // banks).  The group sums of x, with which the offset of the widened codes is taken off, are made beforehand
 // by the kernel that also cuts fp32 activations into their three bf16 pieces or copies rows that are not aligned.
+// A sparse operand comes spread out, with code - zero in its places and zeros between: there are no offsets then and no sums.
 #include "internal.h"
 #include "q4_device.h"
 
@@ -58,7 +59,7 @@ q4_prepare_x_kernel(const void* __restrict__ x_, size_t ldx, int M, int K, int K
         sum += T == kF32 ? __uint_as_float(v[e]) : T == kBF16 ? __uint_as_float(v[e] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)v[e]);
     for (int mask = 1; mask < unit / 8; mask <<= 1)
         sum += __shfl_xor(sum, mask, 64);
-    if (k0 < Kp && (lane & (unit / 8 - 1)) == 0)
+    if (sums && k0 < Kp && (lane & (unit / 8 - 1)) == 0)
         sums[(size_t)(k0 / unit) * sums_ld + row] = sum;
     if (PLANES == 0 || k0 >= Kp)
         return;
@@ -80,9 +81,13 @@ q4_prepare_x_kernel(const void* __restrict__ x_, size_t ldx, int M, int K, int K
     }
 }
 
-// ---- a sparse operand's codes as those of a dense one: the zero point where no row was kept ----------------
+// ---- a sparse operand's codes as a dense operand: a byte a row, zero where none was kept ------------------------
 
-// Bound by its writes (two to eight times its reads); 4096 x 4096 2:4 some 12 us, the price of a sparse operand at 17 rows and more.
+// The byte is an 8-bit float (e4m3) of code - zero: sign and magnitude, whose low numbers are evenly spaced (0 .. 15 stand for
+// 0 .. 15 times 2^-9, exactly).  What x holds in a row that was not kept is multiplied by a zero: it leaves no rounding in the sums.
+// (With the zero point's code there it did, of 31 times its size.)  Layout: [tile][block][half of the
+// steps][lane][step][8 rows], so that a wave stores and reads 1 KB in a piece.
+// Bound by its writes (four to sixteen times its reads); 4096 x 4096 2:4 some 15 us, the price of a sparse operand at 33 rows and more.
 template <int KEPT>     // kept rows that can lie among eight dense ones: those of their windows, or of the one they are part of
 __global__ void __launch_bounds__(256)
 q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict__ meta, const uint8_t* __restrict__ rows,
@@ -93,30 +98,35 @@ q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict
     if (tile >= p.tiles)
         return;
     const int per = 128 / p.group;
-    u32x4 word;
+    u32x4 word[2];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
         const int d0 = min(block * 128 + s * 32 + kb * 8, (p.K - 1) & ~7);  // eight dense rows (of padding: anything, x is zero there)
         const int r0 = d0 / p.m * p.n;                                      // a multiple of KEPT: all in one word
         const size_t at = (size_t)tile * p.blocks + (r0 >> 7);
-        const uint32_t zero = meta[(at * 16 + c) * per + ((r0 >> 5) & 3) * per / 4] & 15u;
+        const int zero = (int)(meta[(at * 16 + c) * per + ((r0 >> 5) & 3) * per / 4] & 15u);
         const uint32_t rotated = codes[(at * 64 + ((r0 >> 3) & 3) * 16 + c) * 4 + ((r0 >> 5) & 3)];
         const uint32_t packed = __builtin_amdgcn_alignbit(rotated, rotated, 3);
         const uint2 eight = *reinterpret_cast<const uint2*>(rows + (size_t)(tile >> 1) * p.blocks * 128 + (r0 & ~7));
         const int base = (r0 >> 5) * p.span - d0;
-        uint32_t dense = zero * 0x11111111u;
+        uint32_t low = 0, high = 0;
 #pragma unroll
         for (int i = 0; i < KEPT; ++i) {
             const int e = (r0 & 7) + i;
             const uint32_t off = ((e < 4 ? eight.x : eight.y) >> (8 * (e & 3))) & 255u;
             const uint32_t d = (uint32_t)(base + (int)off);                 // 0..7 if it is among the eight
-            // what changes from the zero point to the code, put at its place (nibble of row d: 4 (d / 2 + 4 (d % 2)))
-            const uint32_t change = ((packed >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) ^ zero;
-            dense ^= d < 8u && r0 + i < p.W ? change << (2 * (d & 6) + 16 * (d & 1)) : 0u;
+            const int value = (int)((packed >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) - zero;
+            const uint32_t byte = (value < 0 ? 128u : 0u) | (uint32_t)abs(value);
+            const uint32_t there = r0 + i < p.W ? byte << (8 * (d & 3)) : 0u;
+            low |= d < 4u ? there : 0u;
+            high |= d - 4u < 4u ? there : 0u;
         }
-        word[s] = __builtin_amdgcn_alignbit(dense, dense, 29);
+        word[s >> 1][(s & 1) * 2] = low;
+        word[s >> 1][(s & 1) * 2 + 1] = high;
     }
-    *reinterpret_cast<u32x4*>(out + (((size_t)tile * dense_blocks + block) * 64 + lane) * 4) = word;
+    u32x4* const to = reinterpret_cast<u32x4*>(out) + ((size_t)tile * dense_blocks + block) * 128 + lane;
+    to[0] = word[0];
+    to[64] = word[1];
 }
 
 // ---- the product --------------------------------------------------------------------------------------------
@@ -128,14 +138,14 @@ struct GemmArgs {
     size_t plane, ldx;
     const float* sums;      // [K / unit][sums_ld]
     size_t sums_ld;
-    const uint32_t* codes;  // dense
+    const uint32_t* codes;  // dense: 4 bits a row, or 8 (q4_densify_kernel)
     Q4Meta meta;
     const float* bias;
     void* y;
     size_t ldy;
     float* partial;         // [split][M][partial_ld] where K is split
     size_t partial_ld;
-    int M, N, Kx;           // Kx: elements of a row of x, a multiple of 128
+    int M, N;
     int blocks, unit;       // dense blocks of 128 rows; rows after which sums are scaled (32, 64, 128)
     int splits;
     int tiles, tiles_m, tiles_n;    // 16-column tiles of the operand; workgroups along rows and columns
@@ -147,10 +157,13 @@ struct GemmArgs {
 // third of the time; 5.8 vector instructions go with each of theirs (widening 1.3, scales and offsets 2), and a stage waits
 // for its x in LDS.  Wider tiles (two column tiles a wave), offsets as one more product and x a stage further ahead were slower
 // (227 to 249 us).  Groups of 64 / 32 scale two and four times as often: 290 / 480 us; three pieces of fp32 450.
-template <ElementType T, int PLANES, ElementType OUT, int RT, int NC, int STEPS>
+// BYTES: a spread-out operand's, code - zero exactly: sums start from zero and take none of x's.
+template <ElementType T, int PLANES, ElementType OUT, bool BYTES, int RT, int NC, int STEPS>
 __global__ void __launch_bounds__(256, 2)
 q4_gemm_kernel(GemmArgs g)
 {
+    constexpr bool Exact = BYTES;
+    constexpr int Words = BYTES ? 2 : 1;                                    // of a step
     constexpr int Rows = 16 * RT;
     constexpr int StageSteps = PLANES == 1 ? 4 : 2;                         // 32-row steps of a stage
     constexpr int Loops = StageSteps > STEPS ? StageSteps / STEPS : 1;      // units (or the part of one) in a stage
@@ -159,7 +172,7 @@ q4_gemm_kernel(GemmArgs g)
     constexpr int RowBytes = Pieces * 16;
     constexpr int Mine = (Rows * Pieces + 255) / 256;                       // pieces that a thread brings
     __shared__ __attribute__((aligned(16))) unsigned char tile[2][Rows * RowBytes];
-    __shared__ __attribute__((aligned(16))) float sums[2][Loops][Rows];
+    __shared__ __attribute__((aligned(16))) float sums[2][Loops][Exact ? 4 : Rows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, kb = lane >> 4;
 
@@ -209,7 +222,7 @@ q4_gemm_kernel(GemmArgs g)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_u32*)(to + (i * 4 + wave) * 1024), 16, (int)from[i], 0, 0, 0);
     };
     auto fetch_sums = [&](int stage) {
-        if (wave < Loops) {
+        if (!Exact && wave < Loops) {
             const int unit = (stage * StageSteps + wave * LoopSteps) / STEPS;
             const float* const base = g.sums + (size_t)unit * g.sums_ld + m0;
             const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, rows_here * 4, 0x00020000);
@@ -217,21 +230,25 @@ q4_gemm_kernel(GemmArgs g)
         }
     };
     auto put_sums = [&](int half) {
-        if (wave < Loops && lane < Rows)
+        if (!Exact && wave < Loops && lane < Rows)
             sums[half][wave][lane] = __uint_as_float(sr);
     };
-    uint32_t w[NC][StageSteps], wn[NC][StageSteps], mt[NC], mn[NC];
+    uint32_t w[NC][StageSteps * Words], wn[NC][StageSteps * Words], mt[NC], mn[NC];
     auto fetch_codes = [&](int stage) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             const int t = min(tile0 + j, g.tiles - 1);      // beyond the last column: read, not used
             const int b = stage * StageSteps / 4;
-            const uint32_t* const base = g.codes + ((size_t)t * g.blocks + b) * 256 + (PLANES == 1 ? 0 : (stage & 1) * 2) + lane * 4;
-            if (PLANES == 1) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(base);
+            const uint32_t* const base = g.codes + ((size_t)t * g.blocks + b) * (256 * Words) +
+                                         (PLANES == 1 ? 0 : (stage & 1) * (BYTES ? 256 : 2)) + lane * 4;
+            if (PLANES == 1 || BYTES) {
 #pragma unroll
-                for (int s = 0; s < StageSteps; ++s)
-                    wn[j][s] = v[s];
+                for (int h = 0; h < StageSteps * Words / 4; ++h) {
+                    const u32x4 v = reinterpret_cast<const u32x4*>(base)[h * 64];
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+                        wn[j][h * 4 + s] = v[s];
+                }
             } else {
                 const uint2 v = *reinterpret_cast<const uint2*>(base);
                 wn[j][0] = v.x;
@@ -265,8 +282,15 @@ q4_gemm_kernel(GemmArgs g)
                 if (u + 1 < Loops || stage + 1 < end)
                     fetch_meta(stage * StageSteps + (u + 1) * LoopSteps);
             }
-            // a unit's sums start from what its offset takes off, - (16 + zero) times the sum of x
-            if (StageSteps >= STEPS || !(stage & 1)) {
+            // a unit's sums start from what its offset takes off, - (16 + zero) times the sum of x (Exact: from zero)
+            if (Exact) {
+                if (StageSteps >= STEPS || !(stage & 1))
+#pragma unroll
+                    for (int t = 0; t < RT; ++t)
+#pragma unroll
+                        for (int j = 0; j < NC; ++j)
+                            acc[t][j] = f32x4{0, 0, 0, 0};
+            } else if (StageSteps >= STEPS || !(stage & 1)) {
                 f32x4 xs[RT];
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
@@ -287,11 +311,15 @@ q4_gemm_kernel(GemmArgs g)
                 u32x4 wide[NC];
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
-                    uint32_t word = w[j][i];
+                    uint32_t word[Words];
 #pragma unroll
-                    for (int k = 1; k < Loops; ++k)
-                        word = u == k ? w[j][k * LoopSteps + i] : word;
-                    wide[j] = widened<T>(word, one);
+                    for (int h = 0; h < Words; ++h) {
+                        word[h] = w[j][i * Words + h];
+#pragma unroll
+                        for (int k = 1; k < Loops; ++k)
+                            word[h] = u == k ? w[j][(k * LoopSteps + i) * Words + h] : word[h];
+                    }
+                    wide[j] = BYTES ? from_bytes<T>(word[0], word[Words - 1]) : widened<T>(word[0], one);
                 }
 #pragma unroll
                 for (int q = 0; q < PLANES; ++q) {
@@ -333,7 +361,7 @@ q4_gemm_kernel(GemmArgs g)
 #pragma unroll
         for (int j = 0; j < NC; ++j)
 #pragma unroll
-            for (int s = 0; s < StageSteps; ++s)
+            for (int s = 0; s < StageSteps * Words; ++s)
                 w[j][s] = wn[j][s];
         if (Loops == 1)
 #pragma unroll
@@ -392,18 +420,18 @@ q4_gemm_reduce_kernel(const float* __restrict__ partial, size_t partial_ld, int 
             store_result<OUT>(y, (size_t)row * ldy + col + e, sum[e] + (bias ? bias[col + e] : 0.0f));
 }
 
-template <ElementType T, int PLANES, ElementType OUT, int STEPS>
+template <ElementType T, int PLANES, ElementType OUT, bool BYTES, int STEPS>
 void run_steps(const GemmArgs& g, int row_tiles, int column_tiles, hipStream_t stream)
 {
     const dim3 grid(g.tiles_m * g.tiles_n, g.splits);
     if (row_tiles == 1)
-        q4_gemm_kernel<T, PLANES, OUT, 1, 2, STEPS><<<grid, 256, 0, stream>>>(g);
+        q4_gemm_kernel<T, PLANES, OUT, BYTES, 1, 2, STEPS><<<grid, 256, 0, stream>>>(g);
     else if (row_tiles == 2)
-        q4_gemm_kernel<T, PLANES, OUT, 2, 2, STEPS><<<grid, 256, 0, stream>>>(g);
+        q4_gemm_kernel<T, PLANES, OUT, BYTES, 2, 2, STEPS><<<grid, 256, 0, stream>>>(g);
     else if (column_tiles == 2)
-        q4_gemm_kernel<T, PLANES, OUT, 4, 2, STEPS><<<grid, 256, 0, stream>>>(g);
+        q4_gemm_kernel<T, PLANES, OUT, BYTES, 4, 2, STEPS><<<grid, 256, 0, stream>>>(g);
     else
-        q4_gemm_kernel<T, PLANES, OUT, 4, 4, STEPS><<<grid, 256, 0, stream>>>(g);
+        q4_gemm_kernel<T, PLANES, OUT, BYTES, 4, 4, STEPS><<<grid, 256, 0, stream>>>(g);
 }
 
 // How a product is cut: a workgroup's row tiles and column tiles (of a wave), and the ranges of K.
@@ -427,18 +455,18 @@ GemmCut gemm_cut(int M, int tiles, int blocks)
     return c;
 }
 
-template <ElementType T, int PLANES, ElementType OUT>
+template <ElementType T, int PLANES, ElementType OUT, bool BYTES>
 void run_gemm(GemmArgs& g, const GemmCut& c, hipStream_t stream)
 {
     g.tiles_m = c.tiles_m;
     g.tiles_n = c.tiles_n;
     g.splits = c.splits;
     if (g.unit == 128)
-        run_steps<T, PLANES, OUT, 4>(g, c.row_tiles, c.column_tiles, stream);
-    else if (g.unit == 64)
-        run_steps<T, PLANES, OUT, 2>(g, c.row_tiles, c.column_tiles, stream);
+        run_steps<T, PLANES, OUT, BYTES, 4>(g, c.row_tiles, c.column_tiles, stream);
+    else if (BYTES || g.unit == 64)         // (32 kept rows are 64 dense ones and more)
+        run_steps<T, PLANES, OUT, BYTES, 2>(g, c.row_tiles, c.column_tiles, stream);
     else
-        run_steps<T, PLANES, OUT, 1>(g, c.row_tiles, c.column_tiles, stream);
+        run_steps<T, PLANES, OUT, false, 1>(g, c.row_tiles, c.column_tiles, stream);
     if (c.splits > 1)
         q4_gemm_reduce_kernel<OUT><<<dim3(g.M, (g.N + 1023) / 1024), 256, 0, stream>>>(g.partial, g.partial_ld, g.splits, g.bias, g.y,
                                                                                        g.ldy, g.M, g.N);
@@ -457,7 +485,7 @@ static GemmSpace gemm_space(const Q4Shape& p, int M, ElementType type, bool code
     const size_t blocks = ((size_t)p.K + 127) / 128;
     GemmSpace s;
     s.codes = 0;
-    s.sums = codes ? p.tiles * blocks * 1024 : 0;
+    s.sums = codes ? p.tiles * blocks * 2048 : 0;
     s.planes = s.sums;
     s.partial = s.sums;
     s.bytes = s.sums;
@@ -470,12 +498,16 @@ static GemmSpace gemm_space(const Q4Shape& p, int M, ElementType type, bool code
     return s;
 }
 
-bool q4_densifies(const Q4Shape& p, int M) { return p.m > 1 && M > 16; }
+// Rows of a sparse operand that are gathered (q4_linear.hip), sixteen to a launch.  32 rows, 4096 x 4096, us in two such launches / spread
+// out: bf16 2:4 11.3 / 28.9, 2:8 12.9 / 26.4, 1:8 11.0 / 27.6; fp32 2:8 16.3 / 29.7, 1:8 11.7 / 31.2, 2:4 23.7 / 31.9; at 4096 x 11008
+// in groups of 32, fp32 2:4 80 / 52.
+int q4_gathered_rows(const Q4Shape& p, ElementType type) { return type != kF32 || p.m > 2 * p.n || p.group == 128 ? 32 : 16; }
+bool q4_densifies(const Q4Shape& p, int M, ElementType type) { return p.m > 1 && M > q4_gathered_rows(p, type); }
 
 size_t q4_workspace_bytes(const Q4Shape& p, int M, ElementType type)
 {
     // (how 9 to 16 rows are aligned and grouped is not known here)
-    return gemm_space(p, M, type, q4_densifies(p, M), M > (p.m > 1 ? 16 : 8)).bytes;
+    return gemm_space(p, M, type, q4_densifies(p, M, type), M > (p.m > 1 ? q4_gathered_rows(p, type) : 8)).bytes;
 }
 
 hipError_t launch_q4_densify(const Q4LinearArgs& a, uint32_t* out)
@@ -506,7 +538,6 @@ hipError_t launch_q4_gemm(const Q4LinearArgs& a, ElementType type, bool densifie
     g.ldy = a.ldy;
     g.M = a.M;
     g.N = a.p.N;
-    g.Kx = Kp;
     g.blocks = a.p.blocks;
     g.tiles = a.p.tiles;
     g.partial = reinterpret_cast<float*>(base + s.partial);
@@ -516,32 +547,29 @@ hipError_t launch_q4_gemm(const Q4LinearArgs& a, ElementType type, bool densifie
     // x as it is: 16-bit elements, rows of whole blocks on 16-byte boundaries, 64 of them within 1 GiB
     const bool as_is = type != kF32 && a.p.K == Kp && a.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15u) == 0 &&
                        a.ldx < (1u << 23);
-    float* const sums = const_cast<float*>(g.sums);
+    float* const sums = densified ? nullptr : const_cast<float*>(g.sums);
     if (as_is) {
         g.x = static_cast<const uint16_t*>(a.x);
         g.ldx = a.ldx;
         g.plane = 0;
-        if (type == kBF16)
-            q4_prepare_x_kernel<kBF16, 0><<<grid, 256, 0, a.stream>>>(a.x, a.ldx, a.M, a.p.K, Kp, g.unit, nullptr, sums, g.sums_ld);
-        else
-            q4_prepare_x_kernel<kF16, 0><<<grid, 256, 0, a.stream>>>(a.x, a.ldx, a.M, a.p.K, Kp, g.unit, nullptr, sums, g.sums_ld);
     } else {
         g.x = planes;
         g.ldx = type == kF32 ? 3 * (size_t)Kp : Kp;
         g.plane = Kp;
-        if (type == kF32)
-            q4_prepare_x_kernel<kF32, 3><<<grid, 256, 0, a.stream>>>(a.x, a.ldx, a.M, a.p.K, Kp, g.unit, planes, sums, g.sums_ld);
-        else if (type == kBF16)
-            q4_prepare_x_kernel<kBF16, 1><<<grid, 256, 0, a.stream>>>(a.x, a.ldx, a.M, a.p.K, Kp, g.unit, planes, sums, g.sums_ld);
-        else
-            q4_prepare_x_kernel<kF16, 1><<<grid, 256, 0, a.stream>>>(a.x, a.ldx, a.M, a.p.K, Kp, g.unit, planes, sums, g.sums_ld);
     }
+#define NMSPMM_PREPARE(T, PLANES) \
+    q4_prepare_x_kernel<T, PLANES><<<grid, 256, 0, a.stream>>>(a.x, a.ldx, a.M, a.p.K, Kp, g.unit, planes, sums, g.sums_ld)
+    if (!as_is)
+        type == kF32 ? NMSPMM_PREPARE(kF32, 3) : type == kBF16 ? NMSPMM_PREPARE(kBF16, 1) : NMSPMM_PREPARE(kF16, 1);
+    else if (sums)
+        type == kBF16 ? NMSPMM_PREPARE(kBF16, 0) : NMSPMM_PREPARE(kF16, 0);
+#undef NMSPMM_PREPARE
     if (type == kF32)
-        run_gemm<kBF16, 3, kF32>(g, c, a.stream);
+        densified ? run_gemm<kBF16, 3, kF32, true>(g, c, a.stream) : run_gemm<kBF16, 3, kF32, false>(g, c, a.stream);
     else if (type == kBF16)
-        run_gemm<kBF16, 1, kBF16>(g, c, a.stream);
+        densified ? run_gemm<kBF16, 1, kBF16, true>(g, c, a.stream) : run_gemm<kBF16, 1, kBF16, false>(g, c, a.stream);
     else
-        run_gemm<kF16, 1, kF16>(g, c, a.stream);
+        densified ? run_gemm<kF16, 1, kF16, true>(g, c, a.stream) : run_gemm<kF16, 1, kF16, false>(g, c, a.stream);
     return hipGetLastError();
 }
 

@@ -412,7 +412,7 @@ bool few_rows(const Q4LinearArgs& a, ElementType type)
 hipError_t launch_q4_linear(const Q4LinearArgs& given, ElementType type, void* workspace)
 {
     Q4LinearArgs a = given;
-    const bool densified = q4_densifies(a.p, a.M);
+    const bool densified = q4_densifies(a.p, a.M, type);
     if (densified) {
         const hipError_t e = launch_q4_densify(a, static_cast<uint32_t*>(workspace));
         if (e != hipSuccess)
@@ -425,9 +425,21 @@ hipError_t launch_q4_linear(const Q4LinearArgs& given, ElementType type, void* w
         a.p.W = a.p.K;
         a.p.blocks = (a.p.K + 127) / 128;
     }
-    if (!few_rows(a, type))
-        return launch_q4_gemm(a, type, densified, workspace);
     const size_t size = type == kF32 ? 4 : 2;
+    if (a.rows && a.M > 16) {       // sixteen rows at a time (q4_gathered_rows)
+        Q4LinearArgs part = a;
+        for (int first = 0; first < a.M; first += 16) {
+            part.M = a.M - first < 16 ? a.M - first : 16;
+            part.x = static_cast<const char*>(a.x) + first * a.ldx * size;
+            part.y = static_cast<char*>(a.y) + first * a.ldy * size;
+            const hipError_t e = launch_q4_linear(part, type, nullptr);
+            if (e != hipSuccess)
+                return e;
+        }
+        return hipSuccess;
+    }
+    if (densified || !few_rows(a, type))
+        return launch_q4_gemm(a, type, densified, workspace);
     const uintptr_t base = reinterpret_cast<uintptr_t>(a.x);
     // a lane's two neighbouring elements in one load
     const bool pairs = base % (2 * size) == 0 && a.ldx % 2 == 0 && a.p.K % 2 == 0;
