@@ -58,6 +58,24 @@ __device__ inline u32x4 from_bytes(uint32_t low, uint32_t high)
                  __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(high, unit, true))};
 }
 
+// Eight codes -> eight bf16 elements code - zero (exact): 16 + code in fp16, `offset` (twice - (16 + zero) in fp16) added, and to bf16 by way
+// of 8-bit floats, which hold these numbers: two instructions for two of them, where fp32 would take three.
+__device__ inline u32x4 differences(uint32_t w, uint32_t sixteen, uint32_t offset)
+{
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    typedef short i16x2 __attribute__((ext_vector_type(2)));
+    const u32x4 u = widened<kF16>(w, sixteen);
+    u32x4 d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f16x2 two = __builtin_bit_cast(f16x2, (uint32_t)u[i]) + __builtin_bit_cast(f16x2, offset);
+        const i16x2 bytes = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(i16x2{0, 0}, two, 1.0f, false);
+        d[i] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(__builtin_bit_cast(uint32_t, bytes), 1.0f, false));
+    }
+    return d;
+}
+
 template <ElementType T>
 __device__ inline void store_result(void* y, size_t at, float v)
 {

@@ -6,9 +6,12 @@
 // elements, two buffers, 16-byte pieces swapped by row so that the sixteen rows of a read lie in different
 // banks).  The group sums of x, with which the offset of the widened codes is taken off, are made beforehand
 // by the kernel that also cuts fp32 activations into their three bf16 pieces or copies rows that are not aligned.
-// A sparse operand comes spread out, with code - zero in its places and zeros between: there are no offsets then and no sums.
+// A sparse operand comes spread out, with code - zero in its places and zeros between, and for fp32 activations codes
+// are widened to code - zero: there are no offsets then and no sums.
 #include "internal.h"
 #include "q4_device.h"
+
+#include <algorithm>
 
 namespace nmspmm {
 
@@ -88,7 +91,7 @@ q4_prepare_x_kernel(const void* __restrict__ x_, size_t ldx, int M, int K, int K
 // (With the zero point's code there it did, of 31 times its size.)  Layout: [tile][block][half of the
 // steps][lane][step][8 rows], so that a wave stores and reads 1 KB in a piece.
 // Bound by its writes (four to sixteen times its reads); 4096 x 4096 2:4 some 15 us, the price of a sparse operand at 33 rows and more.
-template <int KEPT>     // kept rows that can lie among eight dense ones: those of their windows, or of the one they are part of
+template <int KEPT>     // kept rows that can lie among eight dense ones: those of their windows, or of the one they are part of; 0: dense
 __global__ void __launch_bounds__(256)
 q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict__ meta, const uint8_t* __restrict__ rows,
                   Q4Shape p, int dense_blocks, uint32_t* __restrict__ out)
@@ -107,14 +110,16 @@ q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict
         const int zero = (int)(meta[(at * 16 + c) * per + ((r0 >> 5) & 3) * per / 4] & 15u);
         const uint32_t rotated = codes[(at * 64 + ((r0 >> 3) & 3) * 16 + c) * 4 + ((r0 >> 5) & 3)];
         const uint32_t packed = __builtin_amdgcn_alignbit(rotated, rotated, 3);
-        const uint2 eight = *reinterpret_cast<const uint2*>(rows + (size_t)(tile >> 1) * p.blocks * 128 + (r0 & ~7));
+        uint2 eight = make_uint2(0, 0);
+        if (KEPT)
+            eight = *reinterpret_cast<const uint2*>(rows + (size_t)(tile >> 1) * p.blocks * 128 + (r0 & ~7));
         const int base = (r0 >> 5) * p.span - d0;
         uint32_t low = 0, high = 0;
 #pragma unroll
-        for (int i = 0; i < KEPT; ++i) {
-            const int e = (r0 & 7) + i;
+        for (int i = 0; i < (KEPT ? KEPT : 8); ++i) {
+            const int e = KEPT ? (r0 & 7) + i : i;
             const uint32_t off = ((e < 4 ? eight.x : eight.y) >> (8 * (e & 3))) & 255u;
-            const uint32_t d = (uint32_t)(base + (int)off);                 // 0..7 if it is among the eight
+            const uint32_t d = KEPT ? (uint32_t)(base + (int)off) : i;      // 0..7 if it is among the eight
             const int value = (int)((packed >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) - zero;
             const uint32_t byte = (value < 0 ? 128u : 0u) | (uint32_t)abs(value);
             const uint32_t there = r0 + i < p.W ? byte << (8 * (d & 3)) : 0u;
@@ -156,18 +161,20 @@ struct GemmArgs {
 // 2000 rows of bf16, 4096 x 11008: 217 us, 830 TFLOP/s, where torch's product with bf16 weights takes 288.  The matrix cores are busy a
 // third of the time; 5.8 vector instructions go with each of theirs (widening 1.3, scales and offsets 2), and a stage waits
 // for its x in LDS.  Wider tiles (two column tiles a wave), offsets as one more product and x a stage further ahead were slower
-// (227 to 249 us).  Groups of 64 / 32 scale two and four times as often: 290 / 480 us; three pieces of fp32 450.
-// BYTES: a spread-out operand's, code - zero exactly: sums start from zero and take none of x's.
+// (227 to 249 us).  Groups of 64 / 32 scale two and four times as often: 290 / 480 us; three pieces of fp32 455 (groups of 32: 533).
+// BYTES: a spread-out operand.  There, and with the pieces of an fp32 x, the operand's elements are code - zero exactly: sums start from
+// zero and take none of x's.  (Pieces of 16 + code in one sum lost up to twice as much as an fp32 product does, and what x holds under a zero
+// weight left its rounding; bf16 and fp16 rows of a dense operand, whose results are rounded far coarser, take the cheaper widening.)
 template <ElementType T, int PLANES, ElementType OUT, bool BYTES, int RT, int NC, int STEPS>
 __global__ void __launch_bounds__(256, 2)
 q4_gemm_kernel(GemmArgs g)
 {
-    constexpr bool Exact = BYTES;
+    constexpr bool Exact = BYTES || PLANES == 3;
     constexpr int Words = BYTES ? 2 : 1;                                    // of a step
     constexpr int Rows = 16 * RT;
     constexpr int StageSteps = PLANES == 1 ? 4 : 2;                         // 32-row steps of a stage
-    constexpr int Loops = StageSteps > STEPS ? StageSteps / STEPS : 1;      // units (or the part of one) in a stage
-    constexpr int LoopSteps = StageSteps / Loops;
+    constexpr int Loops = StageSteps / STEPS;                               // units in a stage
+    static_assert(STEPS <= StageSteps, "a unit lies within a stage");
     constexpr int Pieces = PLANES * StageSteps * 4;                         // 16-byte pieces of a row in a stage
     constexpr int RowBytes = Pieces * 16;
     constexpr int Mine = (Rows * Pieces + 255) / 256;                       // pieces that a thread brings
@@ -212,7 +219,7 @@ q4_gemm_kernel(GemmArgs g)
             from[i] = 0x80000000u;      // read as zero
     }
     uint32_t sr = 0;
-    const uint32_t one = sixteens<T>();
+    const uint32_t one = PLANES == 3 ? sixteens<kF16>() : sixteens<T>();
     auto fetch_x = [&](int stage, unsigned char* to) {
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
             const_cast<uint16_t*>(g.x + (size_t)m0 * g.ldx + stage * (StageSteps * 32)), 0, 0x7fffffff, 0x00020000);
@@ -223,7 +230,7 @@ q4_gemm_kernel(GemmArgs g)
     };
     auto fetch_sums = [&](int stage) {
         if (!Exact && wave < Loops) {
-            const int unit = (stage * StageSteps + wave * LoopSteps) / STEPS;
+            const int unit = stage * Loops + wave;
             const float* const base = g.sums + (size_t)unit * g.sums_ld + m0;
             const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, rows_here * 4, 0x00020000);
             sr = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, 0, 0);
@@ -280,17 +287,20 @@ q4_gemm_kernel(GemmArgs g)
                 for (int j = 0; j < NC; ++j)
                     mt[j] = mn[j];
                 if (u + 1 < Loops || stage + 1 < end)
-                    fetch_meta(stage * StageSteps + (u + 1) * LoopSteps);
+                    fetch_meta(stage * StageSteps + (u + 1) * STEPS);
             }
             // a unit's sums start from what its offset takes off, - (16 + zero) times the sum of x (Exact: from zero)
+            uint32_t offset[NC];
+#pragma unroll
+            for (int j = 0; j < NC; ++j)
+                offset[j] = ((mt[j] & 15u) << 6 | 0xcc00u) * 0x10001u;     // - (16 + zero) in fp16, twice
             if (Exact) {
-                if (StageSteps >= STEPS || !(stage & 1))
 #pragma unroll
-                    for (int t = 0; t < RT; ++t)
+                for (int t = 0; t < RT; ++t)
 #pragma unroll
-                        for (int j = 0; j < NC; ++j)
-                            acc[t][j] = f32x4{0, 0, 0, 0};
-            } else if (StageSteps >= STEPS || !(stage & 1)) {
+                    for (int j = 0; j < NC; ++j)
+                        acc[t][j] = f32x4{0, 0, 0, 0};
+            } else {
                 f32x4 xs[RT];
 #pragma unroll
                 for (int t = 0; t < RT; ++t)
@@ -306,8 +316,8 @@ q4_gemm_kernel(GemmArgs g)
                 }
             }
 #pragma unroll
-            for (int i = 0; i < LoopSteps; ++i) {
-                const int s = u * LoopSteps + i;
+            for (int i = 0; i < STEPS; ++i) {
+                const int s = u * STEPS + i;
                 u32x4 wide[NC];
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
@@ -317,9 +327,11 @@ q4_gemm_kernel(GemmArgs g)
                         word[h] = w[j][i * Words + h];
 #pragma unroll
                         for (int k = 1; k < Loops; ++k)
-                            word[h] = u == k ? w[j][(k * LoopSteps + i) * Words + h] : word[h];
+                            word[h] = u == k ? w[j][(k * STEPS + i) * Words + h] : word[h];
                     }
-                    wide[j] = BYTES ? from_bytes<T>(word[0], word[Words - 1]) : widened<T>(word[0], one);
+                    wide[j] = BYTES         ? from_bytes<T>(word[0], word[Words - 1])
+                              : PLANES == 3 ? differences(word[0], one, offset[j])
+                                            : widened<T>(word[0], one);
                 }
 #pragma unroll
                 for (int q = 0; q < PLANES; ++q) {
@@ -336,16 +348,14 @@ q4_gemm_kernel(GemmArgs g)
                 }
             }
             // and are scaled when it ends
-            if (StageSteps >= STEPS || (stage & 1)) {
 #pragma unroll
-                for (int j = 0; j < NC; ++j) {
-                    const float scale = __uint_as_float(mt[j] & ~15u);
+            for (int j = 0; j < NC; ++j) {
+                const float scale = __uint_as_float(mt[j] & ~15u);
 #pragma unroll
-                    for (int t = 0; t < RT; ++t)
+                for (int t = 0; t < RT; ++t)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            total[t][j][e] = fmaf(scale, acc[t][j][e], total[t][j][e]);
-                }
+                    for (int e = 0; e < 4; ++e)
+                        total[t][j][e] = fmaf(scale, acc[t][j][e], total[t][j][e]);
             }
         }
     };
@@ -461,12 +471,12 @@ void run_gemm(GemmArgs& g, const GemmCut& c, hipStream_t stream)
     g.tiles_m = c.tiles_m;
     g.tiles_n = c.tiles_n;
     g.splits = c.splits;
-    if (g.unit == 128)
-        run_steps<T, PLANES, OUT, BYTES, 4>(g, c.row_tiles, c.column_tiles, stream);
-    else if (BYTES || g.unit == 64)         // (32 kept rows are 64 dense ones and more)
+    if (PLANES == 1 && g.unit == 128)
+        run_steps<T, PLANES, OUT, BYTES, PLANES == 1 ? 4 : 2>(g, c.row_tiles, c.column_tiles, stream);
+    else if ((BYTES && PLANES == 1) || g.unit == 64)        // (32 kept rows are 64 dense ones and more)
         run_steps<T, PLANES, OUT, BYTES, 2>(g, c.row_tiles, c.column_tiles, stream);
     else
-        run_steps<T, PLANES, OUT, false, 1>(g, c.row_tiles, c.column_tiles, stream);
+        run_steps<T, PLANES, OUT, BYTES && PLANES == 3, 1>(g, c.row_tiles, c.column_tiles, stream);
     if (c.splits > 1)
         q4_gemm_reduce_kernel<OUT><<<dim3(g.M, (g.N + 1023) / 1024), 256, 0, stream>>>(g.partial, g.partial_ld, g.splits, g.bias, g.y,
                                                                                        g.ldy, g.M, g.N);
@@ -476,7 +486,7 @@ size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
 } // namespace
 
-// What lies where in the workspace (bytes): the densified codes, the sums, the pieces of x, the ranges' results.
+// What lies where in the workspace (bytes): the spread-out codes or the sums of x, the pieces of x, the ranges' results.
 struct GemmSpace {
     size_t codes, sums, planes, partial, bytes;
 };
@@ -491,7 +501,7 @@ static GemmSpace gemm_space(const Q4Shape& p, int M, ElementType type, bool code
     s.bytes = s.sums;
     if (product) {
         const GemmCut c = gemm_cut(M, p.tiles, (int)blocks);
-        s.planes = s.sums + round_up(blocks * 4 * round_up(M, 4) * sizeof(float), 256);
+        s.planes = s.sums + (codes || type == kF32 ? 0 : round_up(blocks * 4 * round_up(M, 4) * sizeof(float), 256));
         s.partial = s.planes + (type == kF32 ? 3 : 1) * (size_t)M * blocks * 256;
         s.bytes = s.partial + (c.splits > 1 ? (size_t)c.splits * M * round_up(p.N, 4) * sizeof(float) : 0);
     }
@@ -502,7 +512,13 @@ static GemmSpace gemm_space(const Q4Shape& p, int M, ElementType type, bool code
 // out: bf16 2:4 11.3 / 28.9, 2:8 12.9 / 26.4, 1:8 11.0 / 27.6; fp32 2:8 16.3 / 29.7, 1:8 11.7 / 31.2, 2:4 23.7 / 31.9; at 4096 x 11008
 // in groups of 32, fp32 2:4 80 / 52.
 int q4_gathered_rows(const Q4Shape& p, ElementType type) { return type != kF32 || p.m > 2 * p.n || p.group == 128 ? 32 : 16; }
-bool q4_densifies(const Q4Shape& p, int M, ElementType type) { return p.m > 1 && M > q4_gathered_rows(p, type); }
+// ... and fp32 rows for which the codes of a dense operand are widened by each workgroup, not spread out once (in groups of 128, us: 512
+// rows of 4096 x 4096 67.3 / 72.7, 2000 rows of 4096 x 11008 506 / 459).
+constexpr int kWidenedRows = 1000;
+bool q4_densifies(const Q4Shape& p, int M, ElementType type)
+{
+    return p.m > 1 ? M > q4_gathered_rows(p, type) : type == kF32 && M > kWidenedRows;
+}
 
 size_t q4_workspace_bytes(const Q4Shape& p, int M, ElementType type)
 {
@@ -515,7 +531,11 @@ hipError_t launch_q4_densify(const Q4LinearArgs& a, uint32_t* out)
     const int blocks = (a.p.K + 127) / 128;
     const dim3 grid(blocks, (a.p.tiles + 3) / 4);
     const int kept = a.p.m > 8 ? a.p.n : 8 / a.p.m * a.p.n;
-    auto kernel = kept == 1 ? q4_densify_kernel<1> : kept == 2 ? q4_densify_kernel<2> : kept == 4 ? q4_densify_kernel<4> : q4_densify_kernel<8>;
+    auto kernel = !a.rows     ? q4_densify_kernel<0>
+                  : kept == 1 ? q4_densify_kernel<1>
+                  : kept == 2 ? q4_densify_kernel<2>
+                  : kept == 4 ? q4_densify_kernel<4>
+                              : q4_densify_kernel<8>;
     kernel<<<grid, 256, 0, a.stream>>>(a.codes, a.meta.words, a.rows, a.p, blocks, out);
     return hipGetLastError();
 }
@@ -528,7 +548,8 @@ hipError_t launch_q4_gemm(const Q4LinearArgs& a, ElementType type, bool densifie
     char* const base = static_cast<char*>(workspace);
     const int Kp = a.p.blocks * 128;
     GemmArgs g;
-    g.unit = a.meta.group < 128 ? a.meta.group : 128;
+    // (fp32: scaling twice as often costs less than sums over two stages, 2000 rows 4096 x 11008 469 against 495 us)
+    g.unit = std::min(a.meta.group, type == kF32 ? 64 : 128);
     g.sums = reinterpret_cast<float*>(base + s.sums);
     g.sums_ld = round_up(a.M, 4);
     g.codes = a.codes;
@@ -547,7 +568,7 @@ hipError_t launch_q4_gemm(const Q4LinearArgs& a, ElementType type, bool densifie
     // x as it is: 16-bit elements, rows of whole blocks on 16-byte boundaries, 64 of them within 1 GiB
     const bool as_is = type != kF32 && a.p.K == Kp && a.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15u) == 0 &&
                        a.ldx < (1u << 23);
-    float* const sums = densified ? nullptr : const_cast<float*>(g.sums);
+    float* const sums = densified || type == kF32 ? nullptr : const_cast<float*>(g.sums);
     if (as_is) {
         g.x = static_cast<const uint16_t*>(a.x);
         g.ldx = a.ldx;
