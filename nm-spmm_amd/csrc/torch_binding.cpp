@@ -5,6 +5,7 @@
 // launch each.
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -51,6 +52,21 @@ void require(bool held, const What&... what)
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 const void* at_of(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+// Whether a call must go through the dispatcher: someone else is to see it (a tracer, a dispatch mode, a function transform), or a tensor has
+// no memory of its own (a wrapper, a batched one).  Keys beside those of an ordinary tensor and of autograd say so.
+bool intercepted(std::initializer_list<const Tensor*> given)
+{
+    constexpr c10::DispatchKeySet ours = c10::DispatchKeySet({c10::DispatchKey::Dense, c10::DispatchKey::BackendSelect, c10::DispatchKey::Negative,
+                                                              c10::DispatchKey::ADInplaceOrView}) |
+                                         c10::autograd_dispatch_keyset | c10::autocast_dispatch_keyset;
+    const auto tls = c10::impl::tls_local_dispatch_key_set();
+    c10::DispatchKeySet keys = tls.included_;
+    for (const Tensor* t : given)
+        if (t->defined())
+            keys = keys | t->key_set();
+    return ((keys - tls.excluded_ - ours).raw_repr() & ~c10::full_backend_mask) != 0;
+}
 
 // What lies in memory is what t stands for, and no tangent of forward-mode differentiation is lost.
 Tensor plain(const Tensor& t)
@@ -114,6 +130,16 @@ Tensor quant_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, 
     check("nmspmm_q4_linear", nmspmm_q4_linear(&op, from.const_data_ptr(), ldx, y.data_ptr(), N, (int)M, type,
                                                const_cast<void*>(at_of(workspace)), need, stream_of(x)));
     return y;
+}
+
+// Nothing where the registered operator is to be called in its place.
+OptTensor quant_linear_direct(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& row_offsets, const OptTensor& bias,
+                              int64_t K, int64_t N, int64_t n, int64_t m, int64_t group)
+{
+    const Tensor rows = row_offsets.value_or(Tensor()), plus = bias.value_or(Tensor());
+    if (intercepted({&x, &codes, &scales, &rows, &plus}))
+        return std::nullopt;
+    return quant_linear(x, codes, scales, row_offsets, bias, K, N, n, m, group);
 }
 
 // ---- the norms around a block -----------------------------------------------------------------------------
@@ -370,13 +396,17 @@ std::pair<Tensor, int64_t> gate_of(const Tensor& gate, at::IntArrayRef shape)
     return {gate.expand(shape), 1};
 }
 
-std::tuple<Tensor, OptTensor> block_norm(const Tensor& residual, const OptTensor& branch, const OptTensor& gate, const OptTensor& scale,
-                                         double factor, int64_t post, const OptTensor& post_weight, const OptTensor& post_bias, int64_t pre,
-                                         const OptTensor& pre_weight, const OptTensor& pre_bias, double eps, double weight_offset,
-                                         const std::optional<at::ScalarType>& dtype)
+// Nothing where the registered operators are to be called in its place.
+std::optional<std::tuple<Tensor, OptTensor>> block_norm(const Tensor& residual, const OptTensor& branch, const OptTensor& gate,
+                                                        const OptTensor& scale,
+                                                        double factor, int64_t post, const OptTensor& post_weight, const OptTensor& post_bias,
+                                                        int64_t pre, const OptTensor& pre_weight, const OptTensor& pre_bias, double eps,
+                                                        double weight_offset, const std::optional<at::ScalarType>& dtype)
 {
     Given g = {residual, branch.value_or(Tensor()), gate.value_or(Tensor()), scale.value_or(Tensor()), post_weight.value_or(Tensor()),
                post_bias.value_or(Tensor()), pre_weight.value_or(Tensor()), pre_bias.value_or(Tensor())};
+    if (intercepted({&g[0], &g[1], &g[2], &g[3], &g[4], &g[5], &g[6], &g[7]}))
+        return std::nullopt;
     require(residual.dim() >= 1 && residual.size(-1) >= 1, "rows must have 1 to 16384 features");
     Conf c;
     c.factor = factor;
@@ -402,10 +432,10 @@ std::tuple<Tensor, OptTensor> block_norm(const Tensor& residual, const OptTensor
     if (tracked && at::GradMode::is_enabled()) {
         const auto o = optional_of(g.data(), kGiven);
         auto made = BlockNorm::apply(o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7], c);
-        return {made[0], c.want_out ? OptTensor(made[1]) : std::nullopt};
+        return std::make_tuple(made[0], c.want_out ? OptTensor(made[1]) : std::nullopt);
     }
     auto made = forward_of(g, c, false);
-    return {g[1].defined() ? made[0] : residual, c.want_out ? OptTensor(made[1]) : std::nullopt};
+    return std::make_tuple(g[1].defined() ? made[0] : residual, c.want_out ? OptTensor(made[1]) : std::nullopt);
 }
 
 // The same in pieces, for the operators that tracing front ends see.
@@ -448,6 +478,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     });
     const py::call_guard<py::gil_scoped_release> others;
     m.def("quant_linear", &quant_linear, others);
+    m.def("quant_linear_direct", &quant_linear_direct, others);
     m.def("block_norm", &block_norm, others);
     m.def("block_norm_forward", &block_norm_forward, others);
     m.def("block_norm_backward", &block_norm_backward, others);

@@ -302,10 +302,14 @@ class NMQuantLinear(torch.nn.Module):
     def forward(self, x):
         b = self._buffers
         bias, codes = b["bias"], b["codes"]
-        # eager inference goes straight to the binding; tracing and gradients see the registered operator
-        eager = type(x) is torch.Tensor and not torch.compiler.is_compiling() and not (x.requires_grad and torch.is_grad_enabled())
-        return (_binding().quant_linear if eager else quant_linear)(
-            x, codes, b["scales"], b["row_offsets"], bias, self.in_features, self.out_features, self.n, self.m, self.group)
+        args = (x, codes, b["scales"], b["row_offsets"], bias, self.in_features, self.out_features, self.n, self.m, self.group)
+        # eager inference goes straight to the binding; gradients, tracers, dispatch modes and function transforms (for which it
+        # returns None) see the registered operator
+        if not torch.compiler.is_compiling() and not (x.requires_grad and torch.is_grad_enabled()):
+            y = _binding().quant_linear_direct(*args)
+            if y is not None:
+                return y
+        return quant_linear(*args)
 
     def extra_repr(self):
         return "in_features=%d, out_features=%d, pattern=%d:%d, group=%d, bias=%s" % (
@@ -417,9 +421,11 @@ def block_norm(residual, branch=None, *, gate=None, residual_scale=1.0, post=Non
     if post not in _NORMS or pre not in _NORMS:
         raise ValueError('post and pre are "rms", "layer" or None')
     scale, factor = (residual_scale, 1.0) if isinstance(residual_scale, torch.Tensor) else (None, float(residual_scale))
-    if not torch.compiler.is_compiling() and type(residual) in (torch.Tensor, torch.nn.Parameter):
-        return _binding().block_norm(residual, branch, gate, scale, factor, _NORMS[post], post_weight, post_bias, _NORMS[pre], pre_weight,
+    if not torch.compiler.is_compiling():
+        made = _binding().block_norm(residual, branch, gate, scale, factor, _NORMS[post], post_weight, post_bias, _NORMS[pre], pre_weight,
                                      pre_bias, eps, weight_offset, dtype)
+        if made is not None:        # (tracers, dispatch modes and function transforms see the registered operators)
+            return made
     D = residual.shape[-1]
     if dtype is None:
         dtype = residual.dtype if branch is None else branch.dtype
