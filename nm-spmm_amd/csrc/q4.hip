@@ -179,11 +179,11 @@ q4_pack_kernel(const float* __restrict__ values, const uint8_t* __restrict__ giv
                 low = fminf(low, lows[t][c * V + i]);
                 odd += odds[t][c * V + i];
             }
-            // The smallest scale of 20 significant bits with steps * scale >= what has to be covered: the quotient is near
-            // enough to be a step off at most (steps * scale has 24 bits: exact, and so is the comparison, in double).
+            // The smallest scale of 20 significant bits with steps * scale >= what has to be covered: the quotient (in double: a range may be
+            // twice what a float holds) is near enough to be a step off at most (steps * scale has 24 bits: the comparison is exact).
             const double steps = asymmetric ? 15.0 : 7.0;
             const double need = asymmetric ? (double)top - (double)low : (double)fmaxf(top, -low);
-            uint32_t bits = __float_as_uint((float)need * (asymmetric ? 1.0f / 15.0f : 1.0f / 7.0f)) & ~15u;
+            uint32_t bits = __float_as_uint((float)(need * (asymmetric ? 1.0 / 15.0 : 1.0 / 7.0))) & ~15u;
             if (steps * (double)__uint_as_float(bits) < need)
                 bits += 16;
             else if (bits >= 16 && steps * (double)__uint_as_float(bits - 16) >= need)

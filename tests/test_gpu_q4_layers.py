@@ -1,0 +1,24 @@
+"""Ranges that end at the largest number, scales, codes that are none, layers that were cast, on the GPU."""
+import numpy as np
+import pytest
+
+from test_gpu_q4 import cuda, op, quantized
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.mark.parametrize("group", [32, 128])
+def test_ranges_beyond_the_largest_number(group):
+    """max - min is more than fp32 holds; the scale, a fifteenth of it, is not."""
+    v = np.zeros((200, 5), np.float32)
+    v[:, 0] = np.linspace(-3e38, 3e38, 200)
+    v[:, 1] = np.where(np.arange(200) % 2, 3.4e38, -3.4e38)
+    v[:, 2] = np.where(np.arange(200) % 3, np.finfo(np.float32).max, -np.finfo(np.float32).max)
+    v[:, 3] = np.linspace(-3e38, 1e38, 200)
+    v[:, 4] = np.linspace(0, 3.4e38, 200)
+    for asymmetric in (False, True):
+        got = op().NMQuantOperand.quantize(cuda(v), None, 200, group=group, asymmetric=asymmetric).dense().cpu().numpy()
+        want = quantized(v, group, asymmetric)
+        with np.errstate(over="ignore"):        # (a scale that covers the largest number may stand for more than it)
+            assert np.array_equal(got, want.astype(np.float32))
