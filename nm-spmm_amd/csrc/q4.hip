@@ -201,10 +201,10 @@ q4_pack_kernel(const float* __restrict__ values, const uint8_t* __restrict__ giv
             mt[i] = 0;
             if (column && (size_t)j * p.group < (size_t)p.W) {
                 const uint32_t z = zeros ? zeros[(size_t)j * p.N + col + i] : 8u;
-                // 20 significant bits, to the nearest (ties away from zero; 16-bit scales are exact)
+                // 20 significant bits, to the nearest (ties away from zero; 16-bit scales are exact), but never to infinity
                 const uint32_t bits = __float_as_uint(scales[(size_t)j * p.N + col + i]);
-                const bool odd = (bits & 0x7f800000u) == 0x7f800000u;
-                mt[i] = ((odd ? 0x7fc00000u : bits + 8u) & ~15u) | (z & 15u);
+                const bool odd = (bits & 0x7f800000u) == 0x7f800000u, last = (bits & 0x7ffffff0u) == 0x7f7ffff0u;
+                mt[i] = ((odd ? 0x7fc00000u : last ? bits : bits + 8u) & ~15u) | (z & 15u);
             }
         }
     }

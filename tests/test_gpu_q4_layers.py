@@ -22,3 +22,14 @@ def test_ranges_beyond_the_largest_number(group):
         want = quantized(v, group, asymmetric)
         with np.errstate(over="ignore"):        # (a scale that covers the largest number may stand for more than it)
             assert np.array_equal(got, want.astype(np.float32))
+
+
+def test_scales_are_kept_to_20_bits():
+    """Nearest number of 20 significant bits; the largest numbers do not become infinite."""
+    scale = np.array([[1.0, 1.0 + 2.0 ** -23, 1.0 + 3 * 2.0 ** -22, 0.1, -0.1, np.finfo(np.float32).max, 3.4e-39]], np.float32)
+    codes = np.full((4, 7), 9, np.uint8)
+    got = op().NMQuantOperand.from_codes(cuda(codes), cuda(scale), None, 4).dense().cpu().numpy()
+    f, e = np.frexp(scale[0].astype(np.float64))
+    want = np.ldexp(np.sign(f) * np.floor(np.ldexp(np.abs(f), 20) + 0.5), e - 20)
+    assert np.array_equal(got[0, :5], want[:5].astype(np.float32))
+    assert np.isfinite(got).all() and abs(got[0, 5] / scale[0, 5] - 1) <= 2.0 ** -19
