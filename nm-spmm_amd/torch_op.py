@@ -208,7 +208,9 @@ class NMQuantOperand:
 
     @classmethod
     def from_codes(cls, codes, scale, zero, K, n=1, m=1, rows=None, group=128):
-        """From codes 0..15 [W, N] (W = K * n / m), scale and zero [ceil(W / group), N]; zero None stands for 8."""
+        """From codes 0..15 [W, N] (W = K * n / m), scale and zero 0..15 [ceil(W / group), N]; zero None stands for 8.  Scales are
+        kept to 20 significant bits, to the nearest: those that were 16-bit floats are exact, fp32 ones may change by 2^-20 of
+        themselves.  Looks at all codes and zero points once (a synchronisation), except while a graph is captured."""
         if codes.dim() != 2 or not codes.is_cuda or codes.dtype != torch.uint8 or n < 1 or m < n or \
                 codes.shape[0] != _nm.q4_kept_rows(K, n, m):
             raise ValueError("codes must be a 2-D uint8 CUDA tensor of K * n / m rows")
@@ -220,6 +222,11 @@ class NMQuantOperand:
             raise ValueError("zero must be a tensor %s of whole numbers 0..15 on the device of the codes" % (per_group,))
         rows = operand._rows(rows, codes)
         with _guard(codes):
+            if not torch.cuda.is_current_stream_capturing():
+                if int(codes.max()) > 15:
+                    raise ValueError("codes must be 0..15")
+                if zero is not None and not (zero.min() >= 0 and zero.max() <= 15):
+                    raise ValueError("zero must be 0..15")
             _nm.q4_pack_device(codes.contiguous(), _floats(scale),
                                None if zero is None else zero.to(torch.uint8).contiguous(), rows, operand._struct())
         return operand

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_q4 import cuda, op, quantized
+from test_gpu_q4 import cuda, make, op, quantized
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -33,3 +33,20 @@ def test_scales_are_kept_to_20_bits():
     want = np.ldexp(np.sign(f) * np.floor(np.ldexp(np.abs(f), 20) + 0.5), e - 20)
     assert np.array_equal(got[0, :5], want[:5].astype(np.float32))
     assert np.isfinite(got).all() and abs(got[0, 5] / scale[0, 5] - 1) <= 2.0 ** -19
+
+
+def test_codes_and_zero_points_above_15_are_refused():
+    codes, scale, zero, _, _ = make(3, 256, 64)
+    for at in (0, 256 * 64 - 1):
+        bad = codes.copy().reshape(-1)
+        bad[at] = 16
+        with pytest.raises(ValueError):
+            op().NMQuantOperand.from_codes(cuda(bad.reshape(256, 64)), cuda(scale), cuda(zero), 256)
+    for value in (16, -1, 256):
+        bad = torch.from_numpy(zero.astype(np.int32)).cuda()
+        bad[1, 3] = value
+        with pytest.raises(ValueError):
+            op().NMQuantLinear.from_codes(cuda(codes), cuda(scale), bad, 256)
+    whole = torch.from_numpy(zero.astype(np.int64)).cuda()
+    a, b = (op().NMQuantOperand.from_codes(cuda(codes), cuda(scale), z, 256).dense() for z in (whole, cuda(zero)))
+    assert torch.equal(a, b)
