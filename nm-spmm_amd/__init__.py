@@ -313,6 +313,8 @@ def q4_operand(codes, meta, row_offsets, K, N, n=1, m=1, group=128, bias=None):
         if t is not None and t.numel() * t.element_size() < need:
             raise ValueError("q4_operand: %s holds %d bytes, the shape arguments need %d"
                              % (name, t.numel() * t.element_size(), need))
+    if bias is not None and not (bias.is_floating_point() and bias.element_size() == 4 and bias.is_contiguous()):
+        raise ValueError("q4_operand: bias must be contiguous float32")
     at = [None if t is None else t.data_ptr() for t in (codes, meta, row_offsets, bias)]
     return Q4Operand(*at, K, N, n, m, group)
 

@@ -295,15 +295,18 @@ class NMQuantLinear(torch.nn.Module):
         self.register_buffer("row_offsets", operand.row_offsets)
         self.register_buffer("bias", None if bias is None else _floats(bias.detach()))
 
-    def _operand(self):
+    def _operand(self, add_bias=True):
         b = self._buffers
-        return _nm.q4_operand(b["codes"], b["scales"], b["row_offsets"], self.in_features, self.out_features, self.n, self.m, self.group, b["bias"])
+        bias = _floats(b["bias"]) if add_bias and b["bias"] is not None else None     # (.to() may have cast it)
+        operand = _nm.q4_operand(b["codes"], b["scales"], b["row_offsets"], self.in_features, self.out_features, self.n, self.m, self.group, bias)
+        operand.keeps = bias
+        return operand
 
     def dense_weight(self):
         """The weight as a dense float32 [out_features, in_features] tensor."""
         out = torch.empty((self.in_features, self.out_features), dtype=torch.float32, device=self.codes.device)
         with _guard(out):
-            _nm.q4_expand_device(self._operand(), out)
+            _nm.q4_expand_device(self._operand(add_bias=False), out)
         return out.t().contiguous()
 
     def forward(self, x):

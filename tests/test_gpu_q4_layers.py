@@ -1,7 +1,10 @@
 """Ranges that end at the largest number, scales, codes that are none, layers that were cast, on the GPU."""
+import copy
+
 import numpy as np
 import pytest
 
+from conftest import nmspmm
 from test_gpu_q4 import cuda, make, op, quantized
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +53,20 @@ def test_codes_and_zero_points_above_15_are_refused():
     whole = torch.from_numpy(zero.astype(np.int64)).cuda()
     a, b = (op().NMQuantOperand.from_codes(cuda(codes), cuda(scale), z, 256).dense() for z in (whole, cuda(zero)))
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+@pytest.mark.parametrize("n,m", [(1, 1), (2, 4)])
+def test_a_cast_layer_still_shows_its_weight(dtype, n, m):
+    w = torch.randn((64, 256), device="cuda")
+    layer = op().NMQuantLinear(w, n, m, bias=torch.randn(64, device="cuda"))
+    weight = layer.dense_weight()
+    cast = copy.deepcopy(layer).to(dtype)
+    assert cast.bias.dtype == dtype
+    assert torch.equal(cast.dense_weight(), weight)
+    # the struct names a float32 bias or none
+    x, y = torch.randn((3, 256), device="cuda"), torch.empty((3, 64), device="cuda")
+    operand = cast._operand()
+    nmspmm.q4_linear(operand, x, y, 3, nmspmm.F32)
+    assert torch.equal(y, cast(x))
+    torch.testing.assert_close(y, x @ weight.t() + cast.bias.float(), rtol=1e-4, atol=1e-3)
