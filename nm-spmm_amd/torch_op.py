@@ -468,7 +468,7 @@ class NMBlockStack(torch.nn.Module):
         count = len(self.blocks)
 
         def vectors(n, value):
-            return torch.nn.ParameterList([torch.nn.Parameter(torch.full((features,), value, device=device)) for _ in range(n)])
+            return torch.nn.ParameterList([torch.nn.Parameter(torch.full((features,), float(value), device=device)) for _ in range(n)])
 
         self.pre_weight, self.post_weight = vectors(count + 1, 1.0), vectors(count, 1.0)
         self.pre_bias = vectors(count + 1, 0.0) if norm == "layer" else None
