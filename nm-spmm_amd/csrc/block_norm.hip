@@ -588,9 +588,8 @@ struct FinishArgs {
     const float* partial;
     void* out[6];
     int type[6], slot[6];
-    int outputs;        // of a whole column each; the gate, if it is here, is the last
-    int gate;           // its place among them, -1 if it is not here
-    int gates, per_gate;
+    int gate;           // the gate's place among the outputs, the last; -1 if it is not here
+    int per_gate;
     int walkers, D;
 };
 __global__ void __launch_bounds__(1024)
@@ -723,7 +722,6 @@ hipError_t launch_block_norm_backward(const BlockNormArgs& a, const BlockNormGra
     FinishArgs f = {};
     f.partial = d.partial;
     f.gate = -1;
-    f.gates = 1;
     f.walkers = w.walkers;
     f.D = a.D;
     int slots = 0;
@@ -746,10 +744,9 @@ hipError_t launch_block_norm_backward(const BlockNormArgs& a, const BlockNormGra
     int outputs = slots;
     if (d.gate && w.per_gate > 1) {
         f.gate = slots;
-        f.gates = (int)((a.rows + a.gate_rows - 1) / a.gate_rows);
         f.per_gate = w.per_gate;
         column(d.gate, a.gate.type, d.slot_gate);
-        outputs += f.gates;
+        outputs += (int)((a.rows + a.gate_rows - 1) / a.gate_rows);
     }
     if (a.rows > 0) {
 #define NMSPMM_TYPES(T, R) backward<T, R>(a, d, w, stream)
