@@ -14,7 +14,7 @@
 //         the low four.
 //   rows  [N / 32][blocks * 128] uint8 (n < m only): the dense row of each kept row, counted from the
 //         first row of the windows of its k-step (32 kept rows span 32 m / n <= 256 dense rows).
-// Rows beyond W and columns beyond N are filled in (the group's zero point, meta 0, offset 0).
+// Rows beyond W and columns beyond N are filled in (the group's zero point, meta 0, the dense row K).
 #include "internal.h"
 
 namespace nmspmm {
@@ -133,9 +133,12 @@ q4_pack_kernel(const float* __restrict__ values, const uint8_t* __restrict__ giv
         row_offsets(local, r0, p, offset, keep);
         if (column && (col & 31) == 0) {
             uint2 eight = make_uint2(0, 0);
+            // rows beyond W name the first element behind x's row, which reads as zero (a step that they share with others spans at most
+            // 256 dense rows and is not whole: 255 at most)
+            const int behind = max(p.K - (r0 >> 5) * p.span, 0);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint32_t byte = r0 + e < p.W ? (uint32_t)offset[e] & 255u : 0u;
+                const uint32_t byte = (uint32_t)(r0 + e < p.W ? offset[e] : behind) & 255u;
                 if (e < 4)
                     eight.x |= byte << (8 * (e & 3));
                 else

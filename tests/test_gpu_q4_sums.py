@@ -125,3 +125,23 @@ def test_sparse_rows_replay_in_a_graph_and_share_no_workspace(n, m, dtype):
             g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(ys, want))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("n,m,windows", [(1, 8, 37), (2, 8, 37), (2, 4, 85), (4, 8, 43), (8, 64, 13), (1, 2, 39), (1, 4, 1), (8, 16, 5), (2, 4, 86)])
+@pytest.mark.parametrize("M", [1, 4, 8, 13, 32, 40])
+def test_what_fills_the_last_step_reads_no_dropped_row(M, n, m, windows, dtype):
+    """W is no multiple of 32: the kept rows of the last step are filled up.  The first dense row of that step is dropped by some vectors."""
+    K, N = windows * m, 256
+    made = make(M + m, K, N, n, m, 32)
+    rows = made[3].reshape(windows, n, N // 32)
+    window = windows * n // 32 * 32 // n
+    drops = ~(rows[window] == 0).any(0)
+    assert drops.any()
+    layer = layer_of(made, K, n, m, 32)
+    keep = torch.from_numpy(np.repeat(drops, 32)).cuda()
+    x = torch.randn((M, K), device="cuda").to(DTYPES[dtype])
+    y = layer(x)
+    for value in (0.0, 6e4, -777.0):
+        x[:, window * m] = value
+        assert torch.equal(layer(x)[:, keep], y[:, keep])
