@@ -362,7 +362,7 @@ size_t nmspmm_q4_row_offsets_bytes(int K, int N, int n, int m);
 int nmspmm_q4_quantize_device(const float* dBT, const int32_t* dDT, const nmspmm_q4_operand* op,
                               unsigned flags, void* stream);
 /* The same from codes that exist already (an imported checkpoint): d_codes[W][N], one code per byte
- * (the low four bits count), d_scales[ceil(W / group)][N] (kept to 20 significant bits: scales that
+ * (the low four bits count; the torch layer refuses codes and zero points above 15), d_scales[ceil(W / group)][N] (kept to 20 significant bits: scales that
  * were 16-bit floats are exact), d_zeros like d_scales, one 0 .. 15 per byte, or NULL for 8. */
 int nmspmm_q4_pack_device(const uint8_t* d_codes, const float* d_scales, const uint8_t* d_zeros,
                           const int32_t* dDT, const nmspmm_q4_operand* op, void* stream);
@@ -371,8 +371,17 @@ int nmspmm_q4_expand_device(const nmspmm_q4_operand* op, float* dB, void* stream
 
 /* y[M][N] = x[M][K] B + bias: rows of x are ldx elements apart (K to 2^24), rows of y ldy (N to 2^24), both of
  * `type`; sums in fp32, one rounding at the end.  M == 0 does nothing.  fp32 activations are multiplied
- * exactly (three bf16 pieces each), so the result is as near as an fp32 product's.  A row of x that
- * holds an infinity or a NaN, or magnitudes beyond 2^100, gives a row of NaN.  x and y must not overlap.
+ * as three bf16 pieces each, exactly.  What else the sums round:
+ *   fp32 rows, more than 16 of a dense operand; more than 32 rows of a sparse one (fp32: m = 2 n in groups below 128,
+ *   more than 16): products are exact, additions round relative to the sums of |x| |B| over what is kept, as
+ *   in an fp32 product;
+ *   all others: a group's zero point is taken off its sums, and additions round relative to 31 * scale * (sum of |x|
+ *   over the group's kept rows).  For ordinary activations that is an fp32 product's accuracy too; an
+ *   activation far larger than the others under a weight of zero leaves its 2^-24 in the result.
+ * Finite activations that the operand does not keep change no bit of a column's result.  An infinity or a NaN
+ * makes its row's results infinite or NaN where it is kept; where it is not kept the result is NaN or what
+ * the kept ones give, depending on the number of rows.  Other rows' results do not change.  Magnitudes up to 2^100 cannot
+ * overflow a group's sums; larger ones may.  x and y must not overlap.
  * The workspace (16-byte aligned) holds what nmspmm_q4_workspace_bytes says, which is 0 for up to 8 rows (it may be NULL
  * then).  Calls that may overlap in time take workspaces of their own;
  * nothing is kept in one from call to call.  No library state: any streams and threads; may be captured into a HIP graph.
@@ -398,8 +407,9 @@ int nmspmm_q4_linear(const nmspmm_q4_operand* op, const void* x, long long ldx, 
  * `factor`; weights and biases: [features], weight_offset is added to both weights.  Each of these NULL: there is
  * none; each has a type of its own.  stats: NULL, or float[rows][4] that the backward pass needs (16-byte aligned).
  * All arithmetic is fp32, with one rounding of each result.  sum may be the residual's memory and out the
- * branch's (with the same leading dimension).  16-byte aligned rows of whole groups of 8 elements are read
- * and written 16 bytes at a time, anything else element by element. */
+ * branch's (with the same leading dimension).  Rows of 8 elements and more are read and written eight elements at a
+ * time, whatever their alignment (the last eight overlap those before where the width is no multiple of 8; only
+ * a row's own last elements are then written one by one), fastest where rows are 16-byte aligned. */
 typedef enum nmspmm_norm { NMSPMM_NORM_NONE = 0, NMSPMM_NORM_RMS = 1, NMSPMM_NORM_LAYER = 2 } nmspmm_norm;
 typedef struct nmspmm_block_norm {
     long long rows, gate_rows, ld_residual, ld_branch, ld_sum, ld_out;

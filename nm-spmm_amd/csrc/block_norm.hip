@@ -379,8 +379,9 @@ block_norm_kernel(BlockNormArgs a, int row_threads, int walkers)
 }
 
 // ---- backward -----------------------------------------------------------------------------------------
-// 4096 rows of 4096 bf16, all six parameters: 49 us (201 MB, 4.1 TB/s) and 6.4 to add the walkers' sums up; 1505 rows of 1536 fp32:
-// 18.5 (55 MB, 3.0 TB/s) and 4.8.
+// 4096 rows of 4096 bf16, all six parameters: 49 us (201 MB and 33.5 MB of walkers' sums, 4.8 TB/s) and 6.4 to add those up; 1505 rows of
+// 1536 fp32: 18.5 (55 MB without the sums, 3.0 TB/s) and 4.8.  Above 4096 features registers do not suffice: 8192 spills some 200 of them, wider
+// rows three to four times as many.
 
 template <ElementType T, ElementType R, bool WIDE, int NV, int THREADS, bool BIAS>
 __global__ void __launch_bounds__(THREADS)

@@ -90,7 +90,7 @@ q4_prepare_x_kernel(const void* __restrict__ x_, size_t ldx, int M, int K, int K
 // 0 .. 15 times 2^-9, exactly).  What x holds in a row that was not kept is multiplied by a zero: it leaves no rounding in the sums.
 // (With the zero point's code there it did, of 31 times its size.)  Layout: [tile][block][half of the
 // steps][lane][step][8 rows], so that a wave stores and reads 1 KB in a piece.
-// Bound by its writes (four to sixteen times its reads); 4096 x 4096 2:4 some 15 us, the price of a sparse operand at 33 rows and more.
+// Bound by its writes (four to sixteen times its reads); 4096 x 11008 2:4 29 us, 2:8 20, the price of a sparse operand at 33 rows and more.
 template <int KEPT>     // kept rows that can lie among eight dense ones: those of their windows, or of the one they are part of; 0: dense
 __global__ void __launch_bounds__(256)
 q4_densify_kernel(const uint32_t* __restrict__ codes, const uint32_t* __restrict__ meta, const uint8_t* __restrict__ rows,

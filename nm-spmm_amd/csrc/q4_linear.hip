@@ -8,7 +8,7 @@
 // bf16 and fp16 activations are operands as they are.  An fp32 activation is cut into three bf16 pieces by
 // truncation, 8 + 8 + 8 bits, which is exact; the pieces are rows of the same product (rows 4 i .. 4 i + 2 of a
 // tile for row i of x) and are added at the end, so no activation is rounded.
-// An infinity or a NaN in a row of x makes that row of y NaN.
+// An infinity or a NaN in a row of x makes that row of y NaN in the columns that keep it; what they do not keep is not read into them.
 #include "internal.h"
 #include "q4_device.h"
 

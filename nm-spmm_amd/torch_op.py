@@ -223,10 +223,11 @@ class NMQuantOperand:
         rows = operand._rows(rows, codes)
         with _guard(codes):
             if not torch.cuda.is_current_stream_capturing():
-                if int(codes.max()) > 15:
-                    raise ValueError("codes must be 0..15")
-                if zero is not None and not (zero.min() >= 0 and zero.max() <= 15):
-                    raise ValueError("zero must be 0..15")
+                above = codes.max() > 15
+                if zero is not None:
+                    above = above | (zero.max() > 15) | (zero.min() < 0)
+                if bool(above):
+                    raise ValueError("codes and zero points must be 0..15")
             _nm.q4_pack_device(codes.contiguous(), _floats(scale),
                                None if zero is None else zero.to(torch.uint8).contiguous(), rows, operand._struct())
         return operand
