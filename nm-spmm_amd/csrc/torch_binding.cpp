@@ -438,11 +438,20 @@ std::optional<std::tuple<Tensor, OptTensor>> block_norm(const Tensor& residual, 
     return std::make_tuple(g[1].defined() ? made[0] : residual, c.want_out ? OptTensor(made[1]) : std::nullopt);
 }
 
+// gate_rows 0 stands for all rows, so that a recorded call takes any number of them.
+Conf recorded(const Given& g, Conf c)
+{
+    if (c.gate_rows == 0 && g[0].defined() && g[0].dim() >= 1 && g[0].size(-1) >= 1)
+        c.gate_rows = std::max<int64_t>(g[0].numel() / g[0].size(-1), 1);
+    return c;
+}
+
 // The same in pieces, for the operators that tracing front ends see.
 std::vector<OptTensor> block_norm_forward(const std::vector<OptTensor>& given, double factor, int64_t post, int64_t pre, double eps,
                                           double weight_offset, int64_t gate_rows, at::ScalarType dtype, bool want_out)
 {
-    const auto made = forward_of(given_of(given), Conf{factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out}, true);
+    const Given g = given_of(given);
+    const auto made = forward_of(g, recorded(g, {factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out}), true);
     return optional_of(made.data(), 3);
 }
 
@@ -454,7 +463,8 @@ std::vector<OptTensor> block_norm_backward(const std::vector<OptTensor>& given, 
     std::array<bool, kGiven> which;
     for (int i = 0; i < kGiven; ++i)
         which[i] = i < (int)needs.size() && needs[i];
-    const Given made = backward_of(given_of(given), Conf{factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out}, stats,
+    const Given g = given_of(given);
+    const Given made = backward_of(g, recorded(g, {factor, post, pre, eps, weight_offset, gate_rows, dtype, want_out}), stats,
                                    grad_sum.value_or(Tensor()), grad_out.value_or(Tensor()), which);
     return optional_of(made.data(), kGiven);
 }

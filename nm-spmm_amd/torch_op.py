@@ -395,13 +395,10 @@ _block_norm_op.register_autograd(_block_norm_gradients, setup_context=_block_nor
 
 
 def _gate_rows(gate, shape):
-    """(gate, consecutive rows that share one of its rows) for a gate that broadcasts against `shape`."""
+    """(gate, consecutive rows that share one of its rows, 0 for all) for a gate that broadcasts against `shape`."""
     D = shape[-1]
-    rows = 1
-    for n in shape[:-1]:
-        rows *= n
     if gate.shape == (D,):
-        return gate, rows
+        return gate, 0
     if gate.dim() == len(shape) and gate.shape[-1] == D:
         lead, each = 0, 1
         while lead < len(shape) - 1 and gate.shape[lead] == shape[lead]:
@@ -409,7 +406,7 @@ def _gate_rows(gate, shape):
         for n in shape[lead:-1]:
             each *= n
         if all(n == 1 for n in gate.shape[lead:-1]):
-            return gate, each
+            return gate, max(each, 1)
     return gate.expand(shape), 1
 
 
@@ -440,13 +437,13 @@ def block_norm(residual, branch=None, *, gate=None, residual_scale=1.0, post=Non
     D = residual.shape[-1]
     if dtype is None:
         dtype = residual.dtype if branch is None else branch.dtype
-    gate_rows = residual.numel() // D
+    gate_rows = 0
     if gate is not None:
         gate, gate_rows = _gate_rows(gate, residual.shape)
     if scale is not None and scale.shape != (D,):
         scale = scale.reshape(-1).expand(D)
     total, out, _ = _block_norm_op(residual, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias, factor, _NORMS[post],
-                                   _NORMS[pre], eps, weight_offset, max(gate_rows, 1), dtype, pre is not None)
+                                   _NORMS[pre], eps, weight_offset, gate_rows, dtype, pre is not None)
     return (residual if branch is None else total), (None if pre is None else out)
 
 

@@ -58,6 +58,20 @@ def test_jit_trace_of_the_norms(kind, grad):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("kind", ["none", "feature"])
+def test_a_trace_takes_other_numbers_of_rows(kind):
+    module, lin = norms(kind), layer()
+    traced, traced_lin = torch.jit.trace(module, tuple(inputs())), torch.jit.trace(lin, inputs()[0])
+    for shape in ((2, 7, 96), (3, 10, 96), (1, 1, 96)):
+        x, y = (torch.randn(shape, device="cuda", requires_grad=True) for _ in range(2))
+        got, want = traced(x, y), module(x, y)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        leaves = [x, y, module.pre, module.post]
+        for a, b in zip(*(torch.autograd.grad(r[0].square().sum() + r[1].square().sum(), leaves) for r in (got, want))):
+            torch.testing.assert_close(a, b)
+        assert torch.equal(traced_lin(x.detach()), lin(x.detach()))
+
+
 def test_jit_trace_of_a_first_norm_and_a_stack():
     stack = op().NMBlockStack([torch.nn.Sequential(layer(), torch.nn.SiLU(), op().NMQuantLinear(torch.randn((96, 64), device="cuda")))], 96)
     x, other = inputs()
