@@ -145,3 +145,21 @@ def test_what_fills_the_last_step_reads_no_dropped_row(M, n, m, windows, dtype):
     for value in (0.0, 6e4, -777.0):
         x[:, window * m] = value
         assert torch.equal(layer(x)[:, keep], y[:, keep])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("n,m", [(1, 1), (2, 4), (1, 8)])
+@pytest.mark.parametrize("M", [2, 9, 20, 40, 1030])
+def test_what_is_not_finite_shows_where_it_is_kept_and_in_its_row_alone(M, n, m, value, dtype):
+    K, N = 256, 256
+    made = make(M + m, K, N, n, m)
+    layer = layer_of(made, K, n, m)
+    x = torch.randn((M, K), device="cuda").to(DTYPES[dtype])
+    y = layer(x)
+    at = 3 if n == m else made[3][0, 0]         # of the first window, kept by the first vector
+    x[1, at] = value
+    got = layer(x)
+    keeps = np.ones(N, bool) if n == m else np.repeat((made[3][:n] == at).any(0), 32)
+    assert keeps.any() and not bool(got[1, torch.from_numpy(keeps).cuda()].isfinite().any())
+    assert torch.equal(got[0], y[0]) and torch.equal(got[2:], y[2:])
